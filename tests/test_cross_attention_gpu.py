@@ -328,3 +328,47 @@ def test_compiled():
     got = torch.compile(f, backend="aot_eager", fullgraph=True)(*leaves, rest["lengths"])
     assert torch.equal(got, out)
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, leaves, grad), want))
+
+
+# every form of the two backward kernels: up to 32 rows a head of keys and more, up to 32 keys and more, keys and rows in one piece and in several
+@pytest.mark.parametrize("exponent", [-17, -13, -7, 6, 12])
+@pytest.mark.parametrize(
+    "shape", [(2, 1, 2, 1, 1, 128), (2, 1, 60, 4, 2, 16), (2, 12, 3000, 2, 1, 16), (2, 40, 20, 2, 2, 64), (1, 600, 20, 2, 2, 32), (1, 1100, 300, 2, 1, 64), (1, 100, 2500, 2, 2, 128), (2, 70, 90, 2, 1, 256)], ids=ids
+)
+def test_float16_gradients_of_cotangents_of_any_size(shape, exponent):
+    """Gradients are linear in the cotangent: what is allowed at cotangents of 2^e is what is allowed at 1, times 2^e, and the steps of the
+    results' own type."""
+    B, Lq, Lk, H, Hkv, D = shape
+    t, rest, grad = made(shape, torch.float16, seed=30)
+    # many keys: weights near 1 / Lk, and gradients of q that float16 can hold all the same
+    scale = 1.0 if Lk > 1000 else None
+    if scale:
+        t["q"] = t["q"] / (2 * math.sqrt(D))
+    size = 2.0**exponent
+    grad = (grad.float() * size).half()
+    leaves = {k: v.requires_grad_() for k, v in t.items()}
+    got = torch.autograd.grad(to.cross_attention(**leaves, scale=scale), list(leaves.values()), grad)
+    want = field_oracle.cross_attention(torch.float16, *(v.detach().double() for v in t.values()), None, None, scale, grad.double() / size)
+    for name, g in zip("qkv", got):
+        value, tolerance, narrow = (size * x for x in want[name])
+        fits = value.abs() < 65000
+        assert not g.isnan().any() and not (g.isinf() & fits).any()
+        field_oracle.assert_close(torch.where(fits, g, 0), torch.where(fits, value, 0), tolerance, f"gradient of {name}", narrow, torch.float16)
+
+
+def test_float16_gradients_of_large_cotangents():
+    """Score gradients beyond 65 504 whose sums are not."""
+    g = torch.Generator().manual_seed(31)
+    randn = lambda *s: torch.randn(s, generator=g, dtype=torch.float64)
+    t = dict(q=randn(4, 1, 1, 128) * 0.1, k=randn(4, 2, 1, 128) * 0.5, v=randn(4, 2, 1, 128))
+    t = {k: v.half().cuda().requires_grad_() for k, v in t.items()}
+    grad = (randn(4, 1, 1, 128) * 6000 + 6000 * t["v"][:, :1].detach().cpu().double()).half().cuda()
+    got = torch.autograd.grad(to.cross_attention(**t), list(t.values()), grad)
+    want = field_oracle.cross_attention(torch.float16, *(v.detach().double() for v in t.values()), None, None, None, grad.double())
+    assert all(want[name][0].abs().max() < 65504 for name in "qk")
+    q, k, v = (t[name].detach().cpu().double() for name in "qkv")
+    p = torch.softmax(q[:, 0] @ k[:, :, 0].mT / math.sqrt(128), dim=2)
+    dp = grad.cpu().double()[:, 0] @ v[:, :, 0].mT
+    assert (p * (dp - (p * dp).sum(2, keepdim=True))).abs().max() > 65504
+    for name, x in zip("qk", got):
+        _close(x, want[name], f"gradient of {name}", torch.float16)

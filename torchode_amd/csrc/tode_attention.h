@@ -225,6 +225,38 @@ template <typename T, int NT> __device__ __forceinline__ void keep_low(acc16 *ou
         for (int r = 0; r < 16; ++r) out[t][r] -= (float)(T)out[t][r];
 }
 
+// The power of two that a column's score gradients are taken times ahead of their rounding to T.  They have the size of the
+// cotangent, and float16 has neither its small values (steps stop shrinking at 2^-14) nor its large ones: the largest so far of a column is brought
+// to 2^8, and its sums to another power once one reaches 2^15, as a softmax does with its maximum.  bfloat16 has float32's range.
+template <typename T, int NT> struct ColumnUnit {
+    __device__ __forceinline__ void fit(float *, acc16 *) {}
+    __device__ __forceinline__ float undo() const { return 1; }
+};
+template <int NT> struct ColumnUnit<f16, NT> {
+    unsigned exponent = 0;  // of the power, as float32 has it (127: 1); 0: none yet, all values were zeros
+    static __device__ __forceinline__ float power(unsigned e) { return __uint_as_float(e << 23); }
+    __device__ __forceinline__ void fit(float *m, acc16 *sum) {
+        float top = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(m[r]));
+        top = fmaxf(top, other_half(top));
+        const bool grown = exponent ? top * power(exponent) >= 32768.0f : top > 0;
+        if (__any(grown)) {
+            const int next = min(max(262 - (int)(__float_as_uint(top) >> 23), 4), 250);  // (infinities stay what they are)
+            const float shrink = grown && exponent ? power(next) * power(254 - exponent) : 1;
+            exponent = grown ? next : exponent;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum[t][r] *= shrink;
+        }
+        const float f = power(exponent);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m[r] *= f;
+    }
+    __device__ __forceinline__ float undo() const { return exponent ? power(254 - exponent) : 1; }
+};
+
 // Orders one wavefront's LDS traffic where its lanes hand values to each other.
 __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");

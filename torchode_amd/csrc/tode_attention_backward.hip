@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(64 * WC * WS) attention_dq_kernel(tode_cross_a
         acc16 out[L::NT];
 #pragma unroll
         for (int t = 0; t < L::NT; ++t) out[t] = zero16();
+        ColumnUnit<T, L::NT> unit;
         const int key_tiles = p.scores_matter() ? (p.length + 31) / 32 : 0, per_split = (key_tiles + splits - 1) / splits;
         const int first = split * per_split, last = min(first + per_split, key_tiles);
         for (int t = first; t < last; t += WS) {
@@ -91,8 +92,14 @@ __global__ void __launch_bounds__(64 * WC * WS) attention_dq_kernel(tode_cross_a
                 const float w = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse));
                 ds[r] = bits >> row_of(r, h) & 1 ? w * (dp[r] - total) : 0;
             }
+            unit.fit(ds, out);
             transposed_times<DP>(k_tile, ds, out, lane);
         }
+        const float undo = unit.undo();
+#pragma unroll
+        for (int t = 0; t < L::NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) out[t][r] *= undo;
         if (!join_waves<WS, L::NT>((float *)lds, out, ws, lane) || !there) return;
         const float f = splits > 1 ? 1 : (float)a.scale;
 #pragma unroll
@@ -128,6 +135,7 @@ __global__ void __launch_bounds__(64 * WC * WS) attention_dkv_kernel(tode_cross_
     acc16 dk[L::NT], dv[L::NT];
 #pragma unroll
     for (int t = 0; t < L::NT; ++t) dk[t] = zero16(), dv[t] = zero16();
+    ColumnUnit<T, L::NT> unit;
     const int row_tiles = tile * WC * 32 < p.length ? (p.rows + 31) / 32 : 0, per_split = (row_tiles + splits - 1) / splits;
     const int first = split * per_split, last = min(first + per_split, row_tiles);
     for (int t = first; t < last; t += WS) {
@@ -160,8 +168,14 @@ __global__ void __launch_bounds__(64 * WC * WS) attention_dkv_kernel(tode_cross_
             ds[r] = allowed && p.scores_matter() ? w[r] * fmaf(dp[r], WEIGHT_UNIT<T>, -s_sum[i]) : 0;
         }
         transposed_times<DP>(g_tile, w, dv, lane);
+        unit.fit(ds, dk);
         transposed_times<DP>(q_tile, ds, dk, lane);
     }
+    const float undo = unit.undo();
+#pragma unroll
+    for (int t = 0; t < L::NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dk[t][r] *= undo;
     join_waves<WS, L::NT>((float *)lds, dk, ws, lane);
     if (!join_waves<WS, L::NT>((float *)lds, dv, ws, lane) || key >= p.keys) return;
     const float f = splits > 1 ? 1 : (float)a.scale;
@@ -200,6 +214,7 @@ __device__ __forceinline__ void dkv_tiles(const tode_cross_attention_args &a, co
     acc16 sum[L::NT];
 #pragma unroll
     for (int t = 0; t < L::NT; ++t) sum[t] = zero16();
+    ColumnUnit<T, L::NT> unit;
     const int row_tiles = tile * 128 < p.length && (!KEYS || p.scores_matter()) ? (p.rows + ROWS - 1) / ROWS : 0, per_split = (row_tiles + splits - 1) / splits;
     const int first = split * per_split, last = min(first + per_split, row_tiles);
     Raw<T> q_next[LOADS], g_next[LOADS];
@@ -270,12 +285,13 @@ __device__ __forceinline__ void dkv_tiles(const tode_cross_attention_args &a, co
                 const acc16 dp = rows_times<T, DP>(g_sub, v, lane);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) w[r] *= fmaf(dp[r], WEIGHT_UNIT<T>, -s_sum[32 * sub + row_of(r, h)]);
+                unit.fit(w, sum);
             }
             transposed_times<DP>(KEYS ? q_sub : g_sub, w, sum, lane);
         }
     }
     if (key >= p.keys) return;
-    const float f = splits > 1 && KEYS ? 1 : KEYS ? (float)a.scale : WEIGHT_UNIT<T>;
+    const float f = KEYS ? unit.undo() * (splits > 1 ? 1 : (float)a.scale) : WEIGHT_UNIT<T>;
 #pragma unroll
     for (int t = 0; t < L::NT; ++t)
 #pragma unroll
@@ -324,6 +340,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) attention_dq_tiles_ker
     acc16 out[L::NT];
 #pragma unroll
     for (int t = 0; t < L::NT; ++t) out[t] = zero16();
+    ColumnUnit<T, L::NT> unit;
     const int key_tiles = p.scores_matter() ? (p.length + 31) / 32 : 0, per_split = (key_tiles + splits - 1) / splits;
     const int first = split * per_split, last = min(first + per_split, key_tiles);
     const T *const keys = p.key(0), *const values = p.value(0);
@@ -375,10 +392,11 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) attention_dq_tiles_ker
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] = bits >> row_of(r, 0) & 1 ? ds[r] : 0;
         }
+        unit.fit(ds, out);
         transposed_times<DP>(k_tile, ds, out, lane);
     }
     if (!there) return;
-    const float f = splits > 1 ? 1 : (float)a.scale;
+    const float f = unit.undo() * (splits > 1 ? 1 : (float)a.scale);
 #pragma unroll
     for (int t = 0; t < L::NT; ++t)
 #pragma unroll
