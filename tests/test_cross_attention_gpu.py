@@ -372,3 +372,20 @@ def test_float16_gradients_of_large_cotangents():
     assert (p * (dp - (p * dp).sum(2, keepdim=True))).abs().max() > 65504
     for name, x in zip("qk", got):
         _close(x, want[name], f"gradient of {name}", torch.float16)
+
+
+@pytest.mark.parametrize("where", ["q", "k"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(2, 1, 50, 2, 2, 32), (2, 1, 5000, 2, 2, 64), (2, 20, 300, 2, 1, 64), (2, 300, 40, 1, 1, 64), (2, 300, 700, 2, 1, 64), (300, 40, 100, 2, 2, 16)], ids=ids)
+def test_a_row_of_nan_reaches_all_that_it_looks_at(shape, dtype, where):
+    """The weights of a row whose scores hold a NaN are NaN, and so are the gradients of all values it looks at."""
+    B, Lq, Lk, H, Hkv, D = shape
+    t, _, grad = made(shape, DTYPES[dtype], seed=32)
+    t[where][1, 0, 0, 3] = math.nan
+    lengths = torch.full((B,), Lk - 1, device="cuda")
+    leaves = {k: v.requires_grad_() for k, v in t.items()}
+    out = to.cross_attention(**leaves, lengths=lengths)
+    dq, dk, dv = torch.autograd.grad(out, list(leaves.values()), grad)
+    assert out[1, 0, 0].isnan().all() and out[0].isfinite().all()
+    assert dq[1, 0, 0].isnan().all() and dk[1, : Lk - 1, 0].isnan().all() and dv[1, : Lk - 1, 0].isnan().all()
+    assert not dk[1, Lk - 1].any() and not dv[1, Lk - 1].any() and dk[0].isfinite().all() and dv[0].isfinite().all()

@@ -225,6 +225,11 @@ template <typename T, int NT> __device__ __forceinline__ void keep_low(acc16 *ou
         for (int r = 0; r < 16; ++r) out[t][r] -= (float)(T)out[t][r];
 }
 
+// A row's sums of weights l, times 2^m: what it divides by and its log-sum.  Zeros and infinity where no key was met; a NaN stays one, in
+// the gradients as well.
+__device__ __forceinline__ float reciprocal(float l) { return l == 0 ? 0 : 1 / l; }
+__device__ __forceinline__ float log_sum(float m, float l) { return l == 0 ? INFINITY : m + log2f(l); }
+
 // The power of two that a column's score gradients are taken times ahead of their rounding to T.  They have the size of the
 // cotangent, and float16 has neither its small values (steps stop shrinking at 2^-14) nor its large ones: the largest so far of a column is brought
 // to 2^8, and its sums to another power once one reaches 2^15, as a softmax does with its maximum.  bfloat16 has float32's range.

@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(256, CT * DP <= 128 ? 2 : 1) attention_tiles_k
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         const int row = row0 + 32 * ct + lane % 32;
-        const float f = l[ct] > 0 ? 1 / l[ct] : 0;
-        if (a.lse && h == 0 && row < p.rows) a.lse[p.flat(row)] = l[ct] > 0 ? m[ct] + log2f(l[ct]) : INFINITY;
+        const float f = reciprocal(l[ct]);
+        if (a.lse && h == 0 && row < p.rows) a.lse[p.flat(row)] = log_sum(m[ct], l[ct]);
 #pragma unroll
         for (int t = 0; t < L::NT; ++t)
 #pragma unroll
@@ -271,12 +271,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_short_kernel(tode_cro
             transposed_times<DP>(v_tile + sub * L::VALUES, w[sub], out, lane);
         }
         l += other_half(l);
-        const float f = l > 0 ? 1 / l : 0;
+        const float f = reciprocal(l);
 #pragma unroll
         for (int t = 0; t < L::NT; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) out[t][r] *= f;
-        if (a.lse && h == 0 && row < p.rows) a.lse[p.flat(row)] = l > 0 ? m + log2f(l) : INFINITY;
+        if (a.lse && h == 0 && row < p.rows) a.lse[p.flat(row)] = log_sum(m, l);
         write_columns<T, DP>(p, a.out, own, out, row0, lane);
         if (a.out_low) keep_low<T, L::NT>(out), write_columns<T, DP>(p, a.out_low, own, out, row0, lane);
     }
@@ -380,14 +380,14 @@ __global__ void __launch_bounds__(64 * WC * WS) attention_kernel(tode_cross_atte
         store_column<float, L::NT>(to + 2, out, p.D, h);
         return;
     }
-    const float f = l > 0 ? 1 / l : 0;
+    const float f = reciprocal(l);
 #pragma unroll
     for (int t = 0; t < L::NT; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) out[t][r] *= f;
     store_column<T, L::NT>((T *)a.out + p.flat(row) * p.D, out, p.D, h);
     if (a.out_low) keep_low<T, L::NT>(out), store_column<T, L::NT>((T *)a.out_low + p.flat(row) * p.D, out, p.D, h);
-    if (a.lse && h == 0) a.lse[p.flat(row)] = l > 0 ? m + log2f(l) : INFINITY;
+    if (a.lse && h == 0) a.lse[p.flat(row)] = log_sum(m, l);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -551,8 +551,8 @@ __global__ void __launch_bounds__(256) attention_token_kernel(tode_cross_attenti
                 if (part + e < p.D) to[2 + part + e] = out[r][e];
             continue;
         }
-        const float f = l[r] > 0 ? 1 / l[r] : 0;
-        if (a.lse && part == 0) a.lse[p.flat(r)] = l[r] > 0 ? m[r] + log2f(l[r]) : INFINITY;
+        const float f = reciprocal(l[r]);
+        if (a.lse && part == 0) a.lse[p.flat(r)] = log_sum(m[r], l[r]);
 #pragma unroll
         for (int e = 0; e < N; ++e) out[r][e] *= f;
         auto write = [&](void *of) {
@@ -610,10 +610,10 @@ template <typename T> __global__ void __launch_bounds__(256) attention_join_kern
     for (int i = 1; i < parts; ++i) v += s_sum[thread + i * wide];
     const int query = row / G;
     const long long at = (b * a.queries + query) * a.heads + (group - b * a.kv_heads) * G + row - query * G;
-    v *= l > 0 ? 1 / l : 0;
+    v *= reciprocal(l);
     ((T *)a.out)[at * D + d] = (T)v;
     if (a.out_low) ((T *)a.out_low)[at * D + d] = (T)(v - (float)(T)v);
-    if (a.lse && thread == 0) a.lse[at] = l > 0 ? top + log2f(l) : INFINITY;
+    if (a.lse && thread == 0) a.lse[at] = log_sum(top, l);
 }
 
 struct ForwardPlan {
