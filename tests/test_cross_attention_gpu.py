@@ -389,3 +389,22 @@ def test_a_row_of_nan_reaches_all_that_it_looks_at(shape, dtype, where):
     assert out[1, 0, 0].isnan().all() and out[0].isfinite().all()
     assert dq[1, 0, 0].isnan().all() and dk[1, : Lk - 1, 0].isnan().all() and dv[1, : Lk - 1, 0].isnan().all()
     assert not dk[1, Lk - 1].any() and not dv[1, Lk - 1].any() and dk[0].isfinite().all() and dv[0].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(4, 1, 3, 2, 2, 16), (4, 5, 700, 4, 2, 32), (4, 40, 20, 2, 2, 64), (4, 300, 1030, 2, 1, 64)], ids=ids)
+def test_a_single_key_that_a_mask_leaves_has_no_gradient_of_its_score(shape, dtype):
+    """As one of a single length: by the mask alone, and by both."""
+    B, Lq, Lk, H, Hkv, D = shape
+    t, _, grad = made(shape, DTYPES[dtype], seed=33)
+    mask = torch.zeros((B, Lk), dtype=torch.bool, device="cuda")
+    mask[0, 0] = mask[1, Lk - 1] = mask[2, Lk // 2] = mask[3, Lk // 2] = mask[3, Lk - 1] = True
+    for rest, zero in ((dict(mask=mask), [0, 1, 2]), (dict(mask=mask, lengths=torch.tensor([Lk, Lk, Lk, Lk - 1], device="cuda")), [0, 1, 2, 3])):
+        leaves = {k: v.clone().requires_grad_() for k, v in t.items()}
+        out = to.cross_attention(**leaves, **rest)
+        dq, dk, dv = torch.autograd.grad(out, list(leaves.values()), grad)
+        assert not dq[zero].any() and not dk[zero].any() and not dv[~mask].any()
+        assert all(dv[b][mask[b]].any() for b in (0, 1, 2, 3)) and (len(zero) == 4 or (dq[3].any() and dk[3].any()))
+        want = field_oracle.cross_attention(DTYPES[dtype], *(t[k].double() for k in "qkv"), rest.get("lengths"), mask, None, grad.double())
+        for name, got in zip(("out", *"qkv"), (out.detach(), dq, dk, dv)):
+            _close(got, want[name], name, DTYPES[dtype])

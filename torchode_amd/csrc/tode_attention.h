@@ -170,7 +170,21 @@ template <typename T> struct Group {
     }
     __device__ __forceinline__ bool allowed(int key) const { return key < length && (!a.mask || a.mask[b * a.mask_stride + key]); }
     // The weight of a single key is 1 whatever its score: the gradient of scores is zero, and not what rounding leaves of a difference of equals.
-    __device__ __forceinline__ bool scores_matter() const { return length > 1; }
+    // With a mask the keys of the sample are counted until there are two: most often the first step ends it (64 samples of 64 queries over 200 keys,
+    // float32, forward and backward: 68.8 us, 66.8 without the count).  Called by whole wavefronts.
+    __device__ __forceinline__ bool scores_matter(int lane) const {
+        if (!a.mask || length < 2) return length > 1;
+        const uint8_t *const mask = a.mask + b * a.mask_stride;
+        int seen = 0;
+        for (int first = 0; first < length && seen < 2; first += 512) {
+            int k[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) k[u] = mask[min(first + 64 * u + lane, length - 1)];  // (eight loads under way)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) seen += __popcll(__ballot(k[u] && first + 64 * u + lane < length));
+        }
+        return seen > 1;
+    }
     // 32 keys from `first` on, one bit each
     __device__ __forceinline__ unsigned allowed_bits(int first, int lane) const {
         return (unsigned)__ballot(lane < 32 && allowed(first + lane));

@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(64 * WC * WS) attention_dq_kernel(tode_cross_a
 #pragma unroll
         for (int t = 0; t < L::NT; ++t) out[t] = zero16();
         ColumnUnit<T, L::NT> unit;
-        const int key_tiles = p.scores_matter() ? (p.length + 31) / 32 : 0, per_split = (key_tiles + splits - 1) / splits;
+        const int key_tiles = p.scores_matter(lane) ? (p.length + 31) / 32 : 0, per_split = (key_tiles + splits - 1) / splits;
         const int first = split * per_split, last = min(first + per_split, key_tiles);
         for (int t = first; t < last; t += WS) {
             const int at = 32 * (t + (WS > 1 ? ws : 0));
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(64 * WC * WS) attention_dkv_kernel(tode_cross_
     T *const q_tile = (T *)lds + (WS > 1 ? ws * 2 * L::VALUES : 0), *const g_tile = q_tile + L::VALUES;
     float *const s_lse = (float *)((T *)lds + WS * 2 * L::VALUES) + (WS > 1 ? ws * 64 : 0), *const s_sum = s_lse + 32;
     const int key = (tile * WC + wc) * 32 + lane % 32;
-    const bool allowed = key < p.keys && p.allowed(key);
+    const bool allowed = key < p.keys && p.allowed(key), matter = p.scores_matter(lane);
     Operand<T, DP> k, v;
     k.load(allowed ? p.key(key) : nullptr, p.D, h);
     v.load(allowed ? p.value(key) : nullptr, p.D, h);
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(64 * WC * WS) attention_dkv_kernel(tode_cross_
         for (int r = 0; r < 16; ++r) {
             const int i = row_of(r, h);
             w[r] = allowed ? __builtin_amdgcn_exp2f(fmaf(s[r], c, -s_lse[i])) : 0;
-            ds[r] = allowed && p.scores_matter() ? w[r] * fmaf(dp[r], WEIGHT_UNIT<T>, -s_sum[i]) : 0;
+            ds[r] = allowed && matter ? w[r] * fmaf(dp[r], WEIGHT_UNIT<T>, -s_sum[i]) : 0;
         }
         transposed_times<DP>(g_tile, w, dv, lane);
         unit.fit(ds, dk);
@@ -215,7 +215,7 @@ __device__ __forceinline__ void dkv_tiles(const tode_cross_attention_args &a, co
 #pragma unroll
     for (int t = 0; t < L::NT; ++t) sum[t] = zero16();
     ColumnUnit<T, L::NT> unit;
-    const int row_tiles = tile * 128 < p.length && (!KEYS || p.scores_matter()) ? (p.rows + ROWS - 1) / ROWS : 0, per_split = (row_tiles + splits - 1) / splits;
+    const int row_tiles = tile * 128 < p.length && (!KEYS || p.scores_matter(lane)) ? (p.rows + ROWS - 1) / ROWS : 0, per_split = (row_tiles + splits - 1) / splits;
     const int first = split * per_split, last = min(first + per_split, row_tiles);
     Raw<T> q_next[LOADS], g_next[LOADS];
     float row_next = 0;
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) attention_dq_tiles_ker
 #pragma unroll
     for (int t = 0; t < L::NT; ++t) out[t] = zero16();
     ColumnUnit<T, L::NT> unit;
-    const int key_tiles = p.scores_matter() ? (p.length + 31) / 32 : 0, per_split = (key_tiles + splits - 1) / splits;
+    const int key_tiles = p.scores_matter(lane) ? (p.length + 31) / 32 : 0, per_split = (key_tiles + splits - 1) / splits;
     const int first = split * per_split, last = min(first + per_split, key_tiles);
     const T *const keys = p.key(0), *const values = p.value(0);
     Raw<T> k_next[LOADS], v_next[LOADS];
