@@ -977,7 +977,7 @@ typedef struct tode_cross_attention_args {
     int32_t head_dim;
     int64_t batch, queries, keys;
     double scale;
-    const void *q;              /* [B,Lq,H,D]; strides in values of batch, row and head, the last one is 1 */
+    const void *q;              /* [B,Lq,H,D]; strides in values of batch, row and head, none negative, the last one is 1 */
     const void *k, *v;          /* [B,Lk,Hkv,D] */
     int64_t q_strides[3], k_strides[3], v_strides[3], grad_strides[3];
     const void *lengths;        /* [B] int32, or int64 where lengths_are_64 is set; or NULL */

@@ -95,3 +95,37 @@ def test_c_entries_report_what_they_do_not_take():
     for name in ("tode_group_norm", "tode_cross_attention"):
         assert getattr(lib, name + "_workspace_bytes")(zeros, 0) == _lib.E_INVALID and b"bad sizes" in lib.tode_last_error()
         assert getattr(lib, name)(zeros, None) == _lib.E_INVALID
+
+
+def attention_args(**fields):
+    """struct tode_cross_attention_args of one sample of two queries and three keys, float32, without a tensor."""
+    import ctypes as C
+
+    class Args(C.Structure):
+        _fields_ = [(n, C.c_int32) for n in ("dtype", "heads", "kv_heads", "head_dim")] + [(n, C.c_int64) for n in ("batch", "queries", "keys")] + [("scale", C.c_double)]
+        _fields_ += [(n, C.c_void_p) for n in "qkv"] + [(n, C.c_int64 * 3) for n in ("q_strides", "k_strides", "v_strides", "grad_strides")]
+        _fields_ += [("lengths", C.c_void_p), ("mask", C.c_void_p), ("mask_stride", C.c_int64), ("lengths_are_64", C.c_int32), ("reserved", C.c_int32)]
+        _fields_ += [(n, C.c_void_p) for n in ("out", "out_low", "lse", "grad_out", "dq", "dk", "dv", "workspace")] + [("workspace_bytes", C.c_int64)]
+
+    a = Args(dtype=0, heads=1, kv_heads=1, head_dim=8, batch=1, queries=2, keys=3, scale=1.0)
+    for name, value in fields.items():
+        setattr(a, name, type(getattr(a, name))(*value) if isinstance(value, tuple) else value)
+    return a
+
+
+@pytest.mark.parametrize("name", ["q_strides", "k_strides", "v_strides", "grad_strides"])
+def test_c_entry_of_cross_attention_refuses_negative_strides(name):
+    import ctypes as C
+
+    from torchode_amd import _lib
+
+    lib = _lib.load()
+    assert lib.tode_cross_attention_workspace_bytes(C.byref(attention_args(k_strides=(24, 8, 8))), 0) == 0
+    for strides in ((-1, 8, 8), (24, -8, 8), (24, 8, -(2**40))):
+        args = attention_args(**{name: strides})
+        assert lib.tode_cross_attention_workspace_bytes(C.byref(args), 1) == _lib.E_INVALID and b"negative" in lib.tode_last_error()
+        assert lib.tode_cross_attention_backward(C.byref(args), None) == _lib.E_INVALID and b"negative" in lib.tode_last_error()
+        if name != "grad_strides":  # (not read by the forward pass)
+            assert lib.tode_cross_attention_workspace_bytes(C.byref(args), 0) == _lib.E_INVALID
+            assert lib.tode_cross_attention(C.byref(args), None) == _lib.E_INVALID and b"negative" in lib.tode_last_error()
+    assert lib.tode_cross_attention(C.byref(attention_args(mask_stride=-3)), None) == _lib.E_INVALID and b"negative" in lib.tode_last_error()

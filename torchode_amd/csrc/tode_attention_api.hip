@@ -3,7 +3,7 @@
 
 namespace tode {
 
-static int check(const tode_cross_attention_args *a) {
+static int check(const tode_cross_attention_args *a, bool backward) {
     if (!a) return fail(TODE_E_INVALID, "null argument struct");
     if (a->dtype != TODE_F32 && a->dtype != TODE_BF16 && a->dtype != TODE_F16) return fail(TODE_E_UNSUPPORTED, "cross attention is built for float32, bfloat16 and float16 (dtype %d)", a->dtype);
     if (a->batch < 0 || a->queries < 0 || a->keys < 0 || a->kv_heads < 1 || a->heads < 1 || a->heads % a->kv_heads || a->head_dim < 1)
@@ -17,6 +17,10 @@ static int check(const tode_cross_attention_args *a) {
     const long long groups = a->batch * a->kv_heads + 7;
     if (groups > limit || (a->queries * share + 31) / 32 > limit / groups || (a->keys + 31) / 32 > limit / groups || a->batch * a->queries > (limit * 64) / a->heads)
         return fail(TODE_E_UNSUPPORTED, "more than 2^30 tiles");
+    // (a row's place in a tile is a 32-bit number where its stride is below 2^24, which one of less than -2^31 would be too)
+    for (int i = 0; i < 3; ++i)
+        if (a->q_strides[i] < 0 || a->k_strides[i] < 0 || a->v_strides[i] < 0 || (backward && a->grad_strides[i] < 0)) return fail(TODE_E_INVALID, "strides must not be negative");
+    if (a->mask_stride < 0) return fail(TODE_E_INVALID, "strides must not be negative");
     if (!(a->scale - a->scale == 0)) return fail(TODE_E_INVALID, "scale must be finite");
     return TODE_OK;
 }
@@ -28,7 +32,7 @@ extern "C" {
 using namespace tode;
 
 int64_t tode_cross_attention_workspace_bytes(const tode_cross_attention_args *a, int32_t backward) {
-    if (int rc = check(a)) return rc;
+    if (int rc = check(a, backward != 0)) return rc;
     if (a->batch == 0) return 0;
     switch (a->dtype) {
         case TODE_F32: return backward ? attention_backward_bytes_float(*a) : attention_forward_bytes_float(*a);
@@ -38,7 +42,7 @@ int64_t tode_cross_attention_workspace_bytes(const tode_cross_attention_args *a,
 }
 
 static int ready(const tode_cross_attention_args *a, int backward) {
-    if (int rc = check(a)) return rc;
+    if (int rc = check(a, backward != 0)) return rc;
     if (a->batch == 0) return TODE_OK;
     if (a->queries > 0 && (!a->q || !a->out)) return fail(TODE_E_INVALID, "null pointer");
     if (a->keys > 0 && (!a->k || !a->v)) return fail(TODE_E_INVALID, "null pointer");
