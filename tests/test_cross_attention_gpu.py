@@ -408,3 +408,20 @@ def test_a_single_key_that_a_mask_leaves_has_no_gradient_of_its_score(shape, dty
         want = field_oracle.cross_attention(DTYPES[dtype], *(t[k].double() for k in "qkv"), rest.get("lengths"), mask, None, grad.double())
         for name, got in zip(("out", *"qkv"), (out.detach(), dq, dk, dv)):
             _close(got, want[name], name, DTYPES[dtype])
+
+
+@pytest.mark.parametrize("batch,training", [(2**26 + 41, False), (2**24 + 41, True)])
+def test_more_workgroups_than_a_grid_has_in_a_row(batch, training):
+    """2^32 threads and more: as the same samples a part at a time."""
+    g = torch.Generator("cuda").manual_seed(34)
+    t = {k: torch.randn((batch, 2 if k != "q" else 1, 1, 4), generator=g, dtype=torch.float16, device="cuda").requires_grad_(training) for k in "qkv"}
+    grad = torch.randn((batch, 1, 1, 4), generator=g, dtype=torch.float16, device="cuda")
+
+    def run(t, grad):
+        out = to.cross_attention(**t)
+        return [out.detach(), *(torch.autograd.grad(out, list(t.values()), grad) if training else [])]
+
+    whole, step = run(t, grad), 2**23
+    for first in range(0, batch, step):
+        part = run({k: v.detach()[first : first + step].requires_grad_(training) for k, v in t.items()}, grad[first : first + step])
+        assert all(torch.equal(a[first : first + step], b) for a, b in zip(whole, part))

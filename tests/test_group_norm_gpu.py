@@ -274,3 +274,20 @@ def test_compiled():
     out = torch.compile(f, backend="aot_eager", fullgraph=True)(*leaves)
     assert torch.equal(out, y)
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, dy), want))
+
+
+def test_more_workgroups_than_a_grid_has_in_a_row():
+    """2^32 threads and more: as the same samples a part at a time."""
+    batch, step, g = 2**26 + 41, 2**23, torch.Generator("cuda").manual_seed(20)
+    x, dy = (torch.randn((batch, 4), generator=g, dtype=torch.float16, device="cuda") for _ in range(2))
+    scale = torch.randn((batch, 4), generator=g, dtype=torch.float16, device="cuda")
+
+    def run(x, scale, dy):
+        leaves = [x.detach().requires_grad_(), scale.detach().requires_grad_()]
+        y = to.group_norm(leaves[0], 2, scale=leaves[1], activation="silu")
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    whole = run(x, scale, dy)
+    for first in range(0, batch, step):
+        part = run(x[first : first + step], scale[first : first + step], dy[first : first + step])
+        assert all(torch.equal(a[first : first + step], b) for a, b in zip(whole, part))

@@ -302,7 +302,7 @@ __device__ __forceinline__ bool place(const tode_cross_attention_args &a, unsign
     }
     const unsigned g = n / tiles;
     group = g, tile = (int)(n - g * tiles);
-    return true;
+    return group < groups;
 }
 // How many workgroups that takes.
 inline long long placed(const tode_cross_attention_args &a, int tiles) {

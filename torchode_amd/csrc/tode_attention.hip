@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(256, CT * DP <= 128 ? 2 : 1) attention_tiles_k
     T *const buffer = (T *)lds;  // [2][k, v][KEYS][STRIDE]
     long long group;
     int tile;
-    if (!place(a, blockIdx.x, tiles * splits, group, tile)) return;
+    if (!place(a, block_number(), tiles * splits, group, tile)) return;
     const int split = tile % splits;
     tile /= splits;
     const Group<T> p(a, group);
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_short_kernel(tode_cro
     extern __shared__ __align__(16) char lds[];
     long long group;
     int chunk;
-    if (!place(a, blockIdx.x, chunks, group, chunk)) return;
+    if (!place(a, block_number(), chunks, group, chunk)) return;
     const Group<T> p(a, group);
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, h = lane / 32;
     T *const k_tile = (T *)lds, *const v_tile = k_tile + SUBS * L::VALUES, *const own = v_tile + SUBS * L::VALUES + wave * L::VALUES;
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(64 * WC * WS) attention_kernel(tode_cross_atte
     extern __shared__ __align__(16) char lds[];
     long long group;
     int tile;
-    if (!place(a, blockIdx.x, tiles * splits, group, tile)) return;
+    if (!place(a, block_number(), tiles * splits, group, tile)) return;
     const int split = tile % splits;
     tile /= splits;
     const Group<T> p(a, group);
@@ -415,8 +415,8 @@ template <typename T, int R, int WK>
 __global__ void __launch_bounds__(256) attention_token_kernel(tode_cross_attention_args a, int width, int heads, int splits, float *partial) {
     constexpr int N = Raw<T>::N, U = R > 4 ? 2 : 4;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, blocks = a.kv_heads / heads;
-    const unsigned unit = WK > 1 ? blockIdx.x / splits : blockIdx.x * 4 + wave;
-    const int split = WK > 1 ? (int)(blockIdx.x - unit * splits) : 0;
+    const unsigned block = block_number(), unit = WK > 1 ? block / splits : block * 4 + wave;
+    const int split = WK > 1 ? (int)(block - unit * splits) : 0;
     if (unit >= a.batch * blocks) return;  // (WK = 1 only: no barrier follows)
     const long long b = unit / blocks;
     const int part = lane % width * N, head = (int)(unit - b * blocks) * heads + lane / width % heads, slots = 64 / (width * heads), slot = lane / (width * heads);
@@ -662,7 +662,7 @@ template <typename T, int DP, int WC, int WS> static int launch(const tode_cross
     static_assert(bytes <= 160 * 1024, "LDS");
     if (bytes > 64 * 1024)
         if (int rc = check_hip(hipFuncSetAttribute((const void *)attention_kernel<T, DP, WC, WS>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute")) return rc;
-    hipLaunchKernelGGL((attention_kernel<T, DP, WC, WS>), dim3((unsigned)placed(a, p.tiles * p.splits)), dim3(64 * WC * WS), bytes, s, a, p.tiles, p.splits, (float *)a.workspace);
+    hipLaunchKernelGGL((attention_kernel<T, DP, WC, WS>), grid_line(placed(a, p.tiles * p.splits)), dim3(64 * WC * WS), bytes, s, a, p.tiles, p.splits, (float *)a.workspace);
     if (p.splits > 1) {
         const long long rows = p.groups * a.queries * (a.heads / a.kv_heads);
         hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)rows), dim3(256), 0, s, a, p.splits, (const float *)a.workspace);
@@ -676,7 +676,7 @@ template <typename T, int DP, int CT> static int launch_tiles(const tode_cross_a
     static_assert(bytes <= 160 * 1024, "LDS");
     if (bytes > 64 * 1024)
         if (int rc = check_hip(hipFuncSetAttribute((const void *)attention_tiles_kernel<T, DP, CT>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute")) return rc;
-    hipLaunchKernelGGL((attention_tiles_kernel<T, DP, CT>), dim3((unsigned)placed(a, p.tiles * p.splits)), dim3(256), bytes, s, a, p.tiles, p.splits, (float *)a.workspace);
+    hipLaunchKernelGGL((attention_tiles_kernel<T, DP, CT>), grid_line(placed(a, p.tiles * p.splits)), dim3(256), bytes, s, a, p.tiles, p.splits, (float *)a.workspace);
     if (p.splits > 1) {
         const long long rows = p.groups * a.queries * (a.heads / a.kv_heads);
         hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)rows), dim3(256), 0, s, a, p.splits, (const float *)a.workspace);
@@ -697,7 +697,7 @@ template <typename T, int DP, int SUBS> static int launch_short(const tode_cross
         // a wavefront takes two tiles of rows or more where there are a thousand workgroups without it
         const long long most = (row_tiles + WAVES - 1) / WAVES, wanted = (1024 + p.groups - 1) / p.groups;
         const int chunks = (int)(wanted < most ? wanted : most);
-        hipLaunchKernelGGL((attention_short_kernel<T, DP, SUBS, WAVES>), dim3((unsigned)placed(a, chunks)), dim3(64 * WAVES), bytes, s, a, (int)row_tiles, chunks);
+        hipLaunchKernelGGL((attention_short_kernel<T, DP, SUBS, WAVES>), grid_line(placed(a, chunks)), dim3(64 * WAVES), bytes, s, a, (int)row_tiles, chunks);
         return check_hip(hipGetLastError(), "tode_cross_attention launch");
     }
 }
@@ -713,9 +713,9 @@ template <typename T> static int short_keys(int head_dim) { return sizeof(T) == 
 template <typename T, int R> static int launch_token(const tode_cross_attention_args &a, const ForwardPlan &p, hipStream_t s) {
     const long long units = p.groups / p.heads;
     if (p.shared > 1)
-        hipLaunchKernelGGL((attention_token_kernel<T, R, 4>), dim3((unsigned)(units * p.splits)), dim3(256), 0, s, a, p.width, p.heads, p.splits, (float *)a.workspace);
+        hipLaunchKernelGGL((attention_token_kernel<T, R, 4>), grid_line(units * p.splits), dim3(256), 0, s, a, p.width, p.heads, p.splits, (float *)a.workspace);
     else
-        hipLaunchKernelGGL((attention_token_kernel<T, R, 1>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, s, a, p.width, p.heads, 1, (float *)nullptr);
+        hipLaunchKernelGGL((attention_token_kernel<T, R, 1>), grid_line((units + 3) / 4), dim3(256), 0, s, a, p.width, p.heads, 1, (float *)nullptr);
     if (p.splits > 1)
         hipLaunchKernelGGL((attention_join_kernel<T>), dim3((unsigned)(p.groups * a.queries * (a.heads / a.kv_heads))), dim3(256), 0, s, a, p.splits, (const float *)a.workspace);
     return check_hip(hipGetLastError(), "tode_cross_attention launch");

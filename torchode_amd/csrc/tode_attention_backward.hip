@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(64 * WC * WS) attention_dq_kernel(tode_cross_a
     extern __shared__ __align__(16) char lds[];
     long long group;
     int tile;
-    if (!place(a, blockIdx.x, tiles * splits, group, tile)) return;
+    if (!place(a, block_number(), tiles * splits, group, tile)) return;
     const int split = tile % splits;
     tile /= splits;
     const Group<T> p(a, group);
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(64 * WC * WS) attention_dkv_kernel(tode_cross_
     extern __shared__ __align__(16) char lds[];
     long long group;
     int tile;
-    if (!place(a, blockIdx.x, tiles * splits, group, tile)) return;
+    if (!place(a, block_number(), tiles * splits, group, tile)) return;
     const int split = tile % splits;
     tile /= splits;
     const Group<T> p(a, group);
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(256, 2) attention_dkv_tiles_kernel(tode_cross_
     extern __shared__ __align__(16) char lds[];
     long long group;
     int n;
-    if (!place(a, blockIdx.x, 2 * tiles * splits, group, n)) return;
+    if (!place(a, block_number(), 2 * tiles * splits, group, n)) return;
     const Group<T> p(a, group);
     if (n % 2)
         dkv_tiles<T, DP, false>(a, p, n / 2 / splits, n / 2 % splits, splits, row_sums, partial, lds);
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) attention_dq_tiles_ker
     extern __shared__ __align__(16) char lds[];
     long long group;
     int tile;
-    if (!place(a, blockIdx.x, tiles * splits, group, tile)) return;
+    if (!place(a, block_number(), tiles * splits, group, tile)) return;
     const int split = tile % splits;
     tile /= splits;
     const Group<T> p(a, group);
@@ -456,9 +456,9 @@ template <typename T, int DP, int WC, int WS> static int launch_dq(const tode_cr
         if (int rc = check_hip(hipFuncSetAttribute((const void *)attention_dq_kernel<T, DP, WC, WS>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute")) return rc;
     float *const sums = (float *)a.workspace, *const partial = (float *)((char *)a.workspace + p.sums);
     if constexpr (sizeof(T) == 2 && WC == 4)
-        hipLaunchKernelGGL((attention_dq_tiles_kernel<T, DP>), dim3((unsigned)placed(a, p.row_tiles * p.row_splits)), dim3(256), 4 * L::VALUES * sizeof(T), s, a, p.row_tiles, p.row_splits, sums, partial);
+        hipLaunchKernelGGL((attention_dq_tiles_kernel<T, DP>), grid_line(placed(a, p.row_tiles * p.row_splits)), dim3(256), 4 * L::VALUES * sizeof(T), s, a, p.row_tiles, p.row_splits, sums, partial);
     else
-        hipLaunchKernelGGL((attention_dq_kernel<T, DP, WC, WS>), dim3((unsigned)placed(a, p.row_tiles * p.row_splits)), dim3(64 * WC * WS), bytes, s, a, p.row_tiles, p.row_splits, sums, partial);
+        hipLaunchKernelGGL((attention_dq_kernel<T, DP, WC, WS>), grid_line(placed(a, p.row_tiles * p.row_splits)), dim3(64 * WC * WS), bytes, s, a, p.row_tiles, p.row_splits, sums, partial);
     if (p.row_splits > 1) {
         const long long n = a.batch * a.queries * a.heads * a.head_dim;
         hipLaunchKernelGGL((attention_add_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, n, p.row_splits, n, (const float *)partial, (float)a.scale, (T *)a.dq);
@@ -478,10 +478,10 @@ template <typename T, int DP, int WC, int WS> static int launch_dkv(const tode_c
         constexpr int tiles_bytes = 8 * L::VALUES * (int)sizeof(T) + 1024;
         if (tiles_bytes > 64 * 1024)
             if (int rc = check_hip(hipFuncSetAttribute((const void *)attention_dkv_tiles_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, tiles_bytes), "hipFuncSetAttribute")) return rc;
-        hipLaunchKernelGGL((attention_dkv_tiles_kernel<T, DP>), dim3((unsigned)placed(a, 2 * p.key_tiles * p.key_splits)), dim3(256), tiles_bytes, s, a, p.key_tiles, p.key_splits,
+        hipLaunchKernelGGL((attention_dkv_tiles_kernel<T, DP>), grid_line(placed(a, 2 * p.key_tiles * p.key_splits)), dim3(256), tiles_bytes, s, a, p.key_tiles, p.key_splits,
                            (const float *)sums, partial);
     } else
-        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, WC, WS>), dim3((unsigned)placed(a, p.key_tiles * p.key_splits)), dim3(64 * WC * WS), bytes, s, a, p.key_tiles, p.key_splits, (const float *)sums, partial);
+        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, WC, WS>), grid_line(placed(a, p.key_tiles * p.key_splits)), dim3(64 * WC * WS), bytes, s, a, p.key_tiles, p.key_splits, (const float *)sums, partial);
     if (p.key_splits > 1) {
         const long long n = a.batch * a.keys * a.kv_heads * a.head_dim;
         hipLaunchKernelGGL((attention_add_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, n, p.key_splits, 2 * n, (const float *)partial, (float)a.scale, (T *)a.dk);

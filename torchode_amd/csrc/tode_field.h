@@ -63,6 +63,11 @@ __device__ __forceinline__ void pack(Raw<f16> &r, const float *v) {
     for (int i = 0; i < 4; ++i) r.w[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{v[2 * i], v[2 * i + 1]}, f16x2));
 }
 
+// A grid of n workgroups in a row, wrapped where it would pass 2^32 threads (the last line has workgroups beyond the n-th).
+constexpr long long GRID_LINE = 1ll << 22;
+inline dim3 grid_line(long long n) { return n <= GRID_LINE ? dim3((unsigned)n) : dim3((unsigned)GRID_LINE, (unsigned)((n + GRID_LINE - 1) / GRID_LINE)); }
+__device__ __forceinline__ unsigned block_number() { return blockIdx.x + (unsigned)GRID_LINE * blockIdx.y; }
+
 inline int bytes_of(int dtype) { return dtype == TODE_F64 ? 8 : dtype == TODE_F32 ? 4 : 2; }
 inline bool known_field_dtype(int dtype) { return dtype == TODE_F32 || dtype == TODE_F64 || dtype == TODE_BF16 || dtype == TODE_F16; }
 

@@ -201,7 +201,7 @@ __device__ __forceinline__ bool place_sample(unsigned block, unsigned chunks, lo
     }
     const unsigned sample = block / chunks;
     b = sample, chunk = (int)(block - sample * chunks);
-    return true;
+    return b < samples;
 }
 
 // What a thread has to know of its N channels: n = (x - mean) rstd, z = n gain + offset.  SHORT: n = x rstd - mean rstd, whose error of
@@ -271,7 +271,7 @@ template <typename T, int R, bool WRAPPED> struct Resident {
     bool there, active;
     __device__ __forceinline__ Resident(const NormShape &n) {
         int chunk;
-        there = place_sample(blockIdx.x, n.chunks, n.B, b, chunk);
+        there = place_sample(block_number(), n.chunks, n.B, b, chunk);
         lanes = blockDim.x / n.V, j = threadIdx.x % n.V, lane_row = threadIdx.x / n.V;
         active = lane_row < lanes, rows = active ? (int)n.rows : 0;
         chunk0 = chunk * n.chunk, c0 = WRAPPED ? N * j % n.C : chunk0 + N * j, groups = n.chunk / n.width;
@@ -1095,7 +1095,7 @@ template <typename T, int R, bool WRAPPED> static int launch_resident(const tode
     typedef typename Wide<T>::type A;
     const NormShape &n = p.n;
     const size_t bytes = ((size_t)p.threads * Raw<T>::N + (n.chunk / n.width) * 18) * sizeof(A);
-    hipLaunchKernelGGL((norm_resident_kernel<T, R, WRAPPED>), dim3((unsigned)p.blocks), dim3(p.threads), bytes, s, a, n);
+    hipLaunchKernelGGL((norm_resident_kernel<T, R, WRAPPED>), grid_line(p.blocks), dim3(p.threads), bytes, s, a, n);
     return check_hip(hipGetLastError(), "tode_group_norm launch");
 }
 template <typename T, int R, bool WRAPPED> static int launch_resident_backward(const tode_group_norm_args &a, const ResidentPlan &p, hipStream_t s) {
@@ -1104,7 +1104,7 @@ template <typename T, int R, bool WRAPPED> static int launch_resident_backward(c
     const int cols = n.V * Raw<T>::N, pieces = p.threads / cols > 1 ? p.threads / cols : 1;
     const size_t bytes = ((size_t)2 * p.threads * Raw<T>::N + 2 * pieces * cols + 2 * n.chunk + 2 * (n.chunk / n.width)) * sizeof(A);
     A *const products = (A *)a.workspace;
-    hipLaunchKernelGGL((norm_resident_backward_kernel<T, R, WRAPPED>), dim3((unsigned)p.blocks), dim3(p.threads), bytes, s, a, n, products);
+    hipLaunchKernelGGL((norm_resident_backward_kernel<T, R, WRAPPED>), grid_line(p.blocks), dim3(p.threads), bytes, s, a, n, products);
     if (!a.affine_per_sample && (a.dweight || a.dbias))
         hipLaunchKernelGGL((norm_affine_gradients_kernel<A>), dim3((n.C + 15) / 16), dim3(1024), 0, s, a, n.B, n.C, (const A *)products);
     return check_hip(hipGetLastError(), "tode_group_norm_backward launch");
