@@ -291,3 +291,11 @@ def test_more_workgroups_than_a_grid_has_in_a_row():
     for first in range(0, batch, step):
         part = run(x[first : first + step], scale[first : first + step], dy[first : first + step])
         assert all(torch.equal(a[first : first + step], b) for a, b in zip(whole, part))
+
+
+@pytest.mark.parametrize("dtype,channels", [("bf16", 2048), ("f16", 2048), ("f32", 1024), ("f64", 512)])
+def test_as_many_groups_as_channels(dtype, channels):
+    """All channels of a row in one workgroup, each a group of its own."""
+    shape = (1030, (5,), channels, channels)
+    t, dy = made(shape, DTYPES[dtype], params=DTYPES[dtype], modulated=True, seed=21)
+    check(shape, DTYPES[dtype], "silu", t, dy)

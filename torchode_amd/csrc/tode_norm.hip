@@ -14,6 +14,7 @@
 namespace tode {
 
 constexpr int NORM_RESIDENT_THREADS = 512;                   // (256 registers each)
+constexpr int NORM_ROW_VECTORS = 256;                        // of a workgroup's part of a row at most: as many groups as values, two sums of each in LDS
 constexpr int NORM_MOST = 32, NORM_MOST_BACKWARD = 8;  // vectors a thread keeps of a tensor: 128 registers, twice 32 (with 16 only one workgroup fits: 65 us against 55)
 
 struct NormShape {
@@ -303,7 +304,7 @@ template <typename T, int R, bool WRAPPED> struct Resident {
     }
     __device__ __forceinline__ void store(void *of, int i, int left, const A *v) const { Vec<T, N>::store((T *)of + first + i * step + thread_offset, left, v); }
     // Sums over the workgroup by group, into total[0 .. groups-1].  One value a thread where its vector lies in one group, else N.
-    // `buffer`: room for blockDim.x * N values, then 16 a group.
+    // `buffer`: room for blockDim.x * N values, then one a group or wavefront, of which there are more.
     __device__ __forceinline__ void sum_groups(const NormShape &n, const A *v, A *buffer, A *total) const {
         const int threads = blockDim.x;
         const bool one = !WRAPPED && n.width % N == 0;
@@ -319,7 +320,7 @@ template <typename T, int R, bool WRAPPED> struct Resident {
                 for (int i = 0; i < N; ++i) buffer[lane_row * cols + j * N + i] = v[i];
         }
         __syncthreads();
-        const int waves = threads / 64, wave = threadIdx.x / 64, lane = threadIdx.x % 64, share = groups < waves ? min(waves / groups, 16) : 1;
+        const int waves = threads / 64, wave = threadIdx.x / 64, lane = threadIdx.x % 64, share = groups < waves ? waves / groups : 1;
         A *const parts = buffer + threads * N;
         for (int k = wave; k < groups * share; k += waves) {
             const int g = k / share, row = WRAPPED ? n.period * width : width, stride = 64 * share, rows_step = stride / row, rest = stride % row;
@@ -362,7 +363,7 @@ template <typename T, int R, bool WRAPPED> __global__ void __launch_bounds__(NOR
     extern __shared__ __align__(16) char lds[];
     const W w(n);
     if (!w.there) return;
-    A *const buffer = (A *)lds, *const totals = buffer + blockDim.x * N + w.groups * 16;
+    A *const buffer = (A *)lds, *const totals = buffer + blockDim.x * N + max(w.groups, (int)blockDim.x / 64);
     Raw<T> x[R];
     w.load(n, a.x, x);
     A sum[N], mean[N];
@@ -462,7 +463,7 @@ __global__ void __launch_bounds__(NORM_RESIDENT_THREADS) norm_resident_backward_
     // columns over the lanes: `pieces` threads a column, then one a channel
     const int cols = n.V * N, pieces = threads / cols > 1 ? threads / cols : 1;
     A *const s_p = (A *)lds, *const s_q = s_p + threads * N, *const piece_p = s_q + threads * N, *const piece_q = piece_p + pieces * cols;
-    A *const channel_p = piece_q + pieces * cols, *const channel_q = channel_p + n.chunk, *const m1 = channel_q + n.chunk, *const m2 = m1 + w.groups;
+    A *const channel_p = s_p, *const channel_q = s_q, *const m1 = piece_q + pieces * cols, *const m2 = m1 + w.groups;  // (s_p and s_q are read by then)
     if (w.active)
 #pragma unroll
         for (int e = 0; e < N; ++e) s_p[w.lane_row * cols + w.j * N + e] = P[e], s_q[w.lane_row * cols + w.j * N + e] = Q[e];
@@ -1020,7 +1021,7 @@ static ResidentPlan resident_of(const tode_group_norm_args &a, int most) {
     if (g < N) {
         n.period = N / g, n.V = n.C / g, n.chunk = n.C, n.chunks = 1;
         n.rows = (n.S + n.period - 1) / n.period;
-        if (n.V > 256) return p;
+        if (n.V > NORM_ROW_VECTORS) return p;
     } else {
         n.period = 1, n.rows = n.S;
         const int base = n.width / gcd(n.width, N) * N, units = n.C / base;  // the least part, and how many of them there are
@@ -1029,7 +1030,7 @@ static ResidentPlan resident_of(const tode_group_norm_args &a, int most) {
         for (int m = 1; m <= units; ++m) {
             if (units % m) continue;
             const long long vectors = n.S * (m * (base / N));
-            if (m * (base / N) > 256 || vectors > (long long)NORM_RESIDENT_THREADS * most) break;
+            if (m * (base / N) > NORM_ROW_VECTORS || vectors > (long long)NORM_RESIDENT_THREADS * most) break;
             if (best && m * base * bytes_of(a.dtype) > 64 && n.B * (units / m) < 1024) break;
             best = m;
         }
@@ -1094,7 +1095,9 @@ static dim3 grid_of(const NormShape &n, int x) { return dim3(x, (unsigned)(n.B <
 template <typename T, int R, bool WRAPPED> static int launch_resident(const tode_group_norm_args &a, const ResidentPlan &p, hipStream_t s) {
     typedef typename Wide<T>::type A;
     const NormShape &n = p.n;
-    const size_t bytes = ((size_t)p.threads * Raw<T>::N + (n.chunk / n.width) * 18) * sizeof(A);
+    const int groups = n.chunk / n.width, waves = p.threads / 64;
+    const size_t bytes = ((size_t)p.threads * Raw<T>::N + (groups > waves ? groups : waves) + 2 * groups) * sizeof(A);
+    static_assert((NORM_RESIDENT_THREADS + 3 * NORM_ROW_VECTORS) * Raw<T>::N * sizeof(A) <= 64 * 1024, "what a launch may have without asking");
     hipLaunchKernelGGL((norm_resident_kernel<T, R, WRAPPED>), grid_line(p.blocks), dim3(p.threads), bytes, s, a, n);
     return check_hip(hipGetLastError(), "tode_group_norm launch");
 }
@@ -1102,7 +1105,8 @@ template <typename T, int R, bool WRAPPED> static int launch_resident_backward(c
     typedef typename Wide<T>::type A;
     const NormShape &n = p.n;
     const int cols = n.V * Raw<T>::N, pieces = p.threads / cols > 1 ? p.threads / cols : 1;
-    const size_t bytes = ((size_t)2 * p.threads * Raw<T>::N + 2 * pieces * cols + 2 * n.chunk + 2 * (n.chunk / n.width)) * sizeof(A);
+    const size_t bytes = ((size_t)2 * p.threads * Raw<T>::N + 2 * pieces * cols + 2 * (n.chunk / n.width)) * sizeof(A);
+    static_assert((2 * NORM_RESIDENT_THREADS + 4 * NORM_ROW_VECTORS) * Raw<T>::N * sizeof(A) <= 64 * 1024, "what a launch may have without asking");
     A *const products = (A *)a.workspace;
     hipLaunchKernelGGL((norm_resident_backward_kernel<T, R, WRAPPED>), grid_line(p.blocks), dim3(p.threads), bytes, s, a, n, products);
     if (!a.affine_per_sample && (a.dweight || a.dbias))
