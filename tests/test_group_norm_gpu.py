@@ -299,3 +299,22 @@ def test_as_many_groups_as_channels(dtype, channels):
     shape = (1030, (5,), channels, channels)
     t, dy = made(shape, DTYPES[dtype], params=DTYPES[dtype], modulated=True, seed=21)
     check(shape, DTYPES[dtype], "silu", t, dy)
+
+
+@pytest.mark.parametrize("value", [30000.0, 3000.0, -0.0123, 57.0])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize(
+    "shape", [(3, (30,), 16, 2), (2, (45, 53), 120, 12), (200, (45, 53), 40, 4), (2, (131, 129), 24, 3), (3, (37,), 30, 5), (150, (157,), 102, 3), (2, (33,), 1501, 1)], ids=lambda s: "x".join(map(str, (s[0], *s[1], s[2])))
+)
+def test_16_bit_groups_without_spread(shape, dtype, value):
+    """Nothing but the bias is left of values that are all the same, and no gradient of the weight."""
+    B, grid, C, G = shape
+    x = torch.full((B, *grid, C), value, dtype=DTYPES[dtype], device="cuda", requires_grad=True)
+    weight = torch.linspace(-2, 2, C, device="cuda", requires_grad=True)
+    bias = torch.linspace(0, 1, C, device="cuda").to(DTYPES[dtype]).float()
+    y = to.group_norm(x, G, weight, bias)
+    assert torch.equal(y, bias.to(DTYPES[dtype]).expand_as(x))
+    (dw,) = torch.autograd.grad(y, weight, torch.randn_like(y))
+    assert not dw.any()
+    with torch.no_grad():
+        assert torch.equal(to.group_norm(x, G, weight, bias), y)

@@ -9,6 +9,8 @@
 // one, so that a thread that goes down the rows meets the same channels every time and keeps their sums and constants in registers.
 #include <math.h>
 
+#include <type_traits>
+
 #include "tode_field.h"
 
 namespace tode {
@@ -205,11 +207,12 @@ __device__ __forceinline__ bool place_sample(unsigned block, unsigned chunks, lo
     return b < samples;
 }
 
-// What a thread has to know of its N channels: n = (x - mean) rstd, z = n gain + offset.  SHORT: n = x rstd - mean rstd, whose error of
-// a unit of mean / deviation is far below that of values that have 8 or 11 bits.
-template <int N, bool SHORT, typename A> struct Channels {
-    A start[N], rstd[N], gain[N], offset[N];  // start: -mean, SHORT: -mean rstd
-    __device__ __forceinline__ A normal(A x, int i) const { return SHORT ? fma(x, rstd[i], start[i]) : (x + start[i]) * rstd[i]; }
+// What a thread has to know of its N channels: n = (x - mean) rstd, z = n gain + offset.  The mean is taken off first: x rstd - mean rstd would
+// leave a unit of mean rstd, which in a group without spread has sqrt(eps) for its divisor (float16, 30 000 everywhere: 0.5 in place of 0; 37 float16 samples of
+// 45 x 53 x 120 with GELU: 29.9 us, that way 28.4; 128 bfloat16 ones of 64 x 64 x 256 with SiLU 152 either way).
+template <int N, typename A> struct Channels {
+    A mean[N], rstd[N], gain[N], offset[N];
+    __device__ __forceinline__ A normal(A x, int i) const { return (x - mean[i]) * rstd[i]; }
     __device__ __forceinline__ void load(const tode_group_norm_args &a, const NormShape &n, long long b, int c0) {
         channel_parameters<N>(a, n, b, c0, gain, offset);
         int group[N];
@@ -217,7 +220,7 @@ template <int N, bool SHORT, typename A> struct Channels {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const long long g = b * n.G + group[i];
-            rstd[i] = ((const A *)a.rstd)[g], start[i] = -((const A *)a.mean)[g] * (SHORT ? rstd[i] : 1);
+            rstd[i] = ((const A *)a.rstd)[g], mean[i] = ((const A *)a.mean)[g];
         }
     }
 };
@@ -303,9 +306,10 @@ template <typename T, int R, bool WRAPPED> struct Resident {
         }
     }
     __device__ __forceinline__ void store(void *of, int i, int left, const A *v) const { Vec<T, N>::store((T *)of + first + i * step + thread_offset, left, v); }
-    // Sums over the workgroup by group, into total[0 .. groups-1].  One value a thread where its vector lies in one group, else N.
+    // Means over the workgroup by group, into total[0 .. groups-1].  One value a thread where its vector lies in one group, else N.
     // `buffer`: room for blockDim.x * N values, then one a group or wavefront, of which there are more.
-    __device__ __forceinline__ void sum_groups(const NormShape &n, const A *v, A *buffer, A *total) const {
+    // S: what they are taken in there.  Returns them divided by `count`.
+    template <typename S> __device__ __forceinline__ void mean_of_groups(const NormShape &n, const A *v, A *buffer, S count, A *total) const {
         const int threads = blockDim.x;
         const bool one = !WRAPPED && n.width % N == 0;
         const int cols = one ? n.V : n.V * N, width = one ? n.width / N : n.width;
@@ -321,12 +325,12 @@ template <typename T, int R, bool WRAPPED> struct Resident {
         }
         __syncthreads();
         const int waves = threads / 64, wave = threadIdx.x / 64, lane = threadIdx.x % 64, share = groups < waves ? waves / groups : 1;
-        A *const parts = buffer + threads * N;
+        S *const parts = (S *)(buffer + threads * N);
         for (int k = wave; k < groups * share; k += waves) {
             const int g = k / share, row = WRAPPED ? n.period * width : width, stride = 64 * share, rows_step = stride / row, rest = stride % row;
             int e = lane + 64 * (k % share), r = e / row;
             e %= row;
-            A t = 0;
+            S t = 0;
             while (r < lanes) {
                 const int p = WRAPPED ? e / width : 0;
                 t += buffer[r * cols + p * n.C + g * width + (e - p * width)];
@@ -338,9 +342,9 @@ template <typename T, int R, bool WRAPPED> struct Resident {
         }
         __syncthreads();
         for (int g = threadIdx.x; g < groups; g += threads) {
-            A t = parts[g * share];
+            S t = parts[g * share];
             for (int k = 1; k < share; ++k) t += parts[g * share + k];
-            total[g] = t;
+            total[g] = (A)(t / count);
         }
         __syncthreads();
     }
@@ -363,7 +367,10 @@ template <typename T, int R, bool WRAPPED> __global__ void __launch_bounds__(NOR
     extern __shared__ __align__(16) char lds[];
     const W w(n);
     if (!w.there) return;
-    A *const buffer = (A *)lds, *const totals = buffer + blockDim.x * N + max(w.groups, (int)blockDim.x / 64);
+    // Sums of 16-bit values that are all the same are exact in a thread (32 values of 11 bits), and between threads in float64: their mean
+    // has to be theirs to the last bit, as what is left of them is divided by sqrt(eps).
+    typedef typename std::conditional<is_short<T>(), double, A>::type S;
+    A *const buffer = (A *)lds, *const means = (A *)((S *)(buffer + blockDim.x * N) + max(w.groups, (int)blockDim.x / 64)), *const variances = means + w.groups;
     Raw<T> x[R];
     w.load(n, a.x, x);
     A sum[N], mean[N];
@@ -377,14 +384,14 @@ template <typename T, int R, bool WRAPPED> __global__ void __launch_bounds__(NOR
         for (int e = 0; e < N; ++e) sum[e] += v[e];  // (zeros behind the end)
         one_at_a_time();
     }
-    w.sum_groups(n, sum, buffer, totals);
+    w.mean_of_groups(n, sum, buffer, (S)n.S * (S)n.width, means);
     keep_packed<R>(x);
     const A count = (A)n.S * (A)n.width;
     int group[N];
     groups_of<N>(n, w.c0, group);
     const int group0 = w.chunk0 / n.width;
 #pragma unroll
-    for (int e = 0; e < N; ++e) mean[e] = totals[group[e] - group0] / count, sum[e] = 0;
+    for (int e = 0; e < N; ++e) mean[e] = means[group[e] - group0], sum[e] = 0;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int left = w.left(n, i);
@@ -399,19 +406,18 @@ template <typename T, int R, bool WRAPPED> __global__ void __launch_bounds__(NOR
         }
         one_at_a_time();
     }
-    A *const squares = totals + w.groups;
-    w.sum_groups(n, sum, buffer, squares);
+    w.mean_of_groups(n, sum, buffer, count, variances);
     keep_packed<R>(x);
     for (int g = threadIdx.x; g < w.groups; g += blockDim.x) {
         const long long k = w.b * n.G + w.chunk0 / n.width + g;
-        if (a.mean) ((A *)a.mean)[k] = totals[g] / count;
-        if (a.rstd) ((A *)a.rstd)[k] = 1 / sqrt(squares[g] / count + (A)a.eps);
+        if (a.mean) ((A *)a.mean)[k] = means[g];
+        if (a.rstd) ((A *)a.rstd)[k] = 1 / sqrt(variances[g] + (A)a.eps);
     }
     if (!w.active) return;
     A gain[N], shift[N];
     channel_parameters<N>(a, n, w.b, w.c0, gain, shift);
 #pragma unroll
-    for (int e = 0; e < N; ++e) gain[e] *= 1 / sqrt(squares[group[e] - group0] / count + (A)a.eps), shift[e] = is_short<T>() ? fma(-mean[e], gain[e], shift[e]) : shift[e];
+    for (int e = 0; e < N; ++e) gain[e] *= 1 / sqrt(variances[group[e] - group0] + (A)a.eps);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int left = w.left(n, i);
@@ -419,7 +425,7 @@ template <typename T, int R, bool WRAPPED> __global__ void __launch_bounds__(NOR
             A v[N];
             unpack(x[i], v);
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = fma(is_short<T>() ? v[e] : v[e] - mean[e], gain[e], shift[e]);
+            for (int e = 0; e < N; ++e) v[e] = fma(v[e] - mean[e], gain[e], shift[e]);
             activate<N, is_short<T>()>(a.activation, v);
             w.store(a.y, i, left, v);
         }
@@ -440,7 +446,7 @@ __global__ void __launch_bounds__(NORM_RESIDENT_THREADS) norm_resident_backward_
     Raw<T> x[R], dy[R];
     w.load(n, a.x, x);
     w.load(n, a.dy, dy);
-    Channels<N, is_short<T>(), A> ch;
+    Channels<N, A> ch;
     ch.load(a, n, w.b, w.c0);
     A P[N], Q[N];
 #pragma unroll
@@ -730,10 +736,10 @@ template <typename T, int N> __global__ void __launch_bounds__(NORM_THREADS) nor
         for (int i = 0; i < N; ++i) mean[i] = ((const A *)a.mean)[b * n.G + group[i]], rstd[i] = ((const A *)a.rstd)[b * n.G + group[i]];
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) gain[i] *= rstd[i], shift[i] = is_short<T>() ? fma(-mean[i], gain[i], shift[i]) : shift[i];
+    for (int i = 0; i < N; ++i) gain[i] *= rstd[i];
     auto apply = [&](A *v) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = fma(is_short<T>() ? v[i] : v[i] - mean[i], gain[i], shift[i]);
+        for (int i = 0; i < N; ++i) v[i] = fma(v[i] - mean[i], gain[i], shift[i]);
         activate<N, is_short<T>()>(a.activation, v);
     };
     const long long full = limit < N ? 0 : min(last, (limit - N) / stride + 1);
@@ -777,7 +783,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_products_kernel(tode_group_
     for (int i = 0; i < N; ++i) P[i] = Q[i] = 0;
     if (at.active) {
         const T *x = (const T *)a.x + offset, *dy = (const T *)a.dy + offset;
-        Channels<N, is_short<T>(), A> ch;
+        Channels<N, A> ch;
         ch.load(a, n, b, at.c0);
         auto add = [&](A *v, A *h) {
             A z[N];
@@ -887,7 +893,7 @@ __global__ void __launch_bounds__(NORM_THREADS) norm_apply_backward_kernel(tode_
     const long long stride = (long long)n.period * n.C, offset = b * end + at.chunk0 + N * at.j, limit = end - at.chunk0 - N * at.j;
     const T *x = (const T *)a.x + offset, *dy = (const T *)a.dy + offset;
     T *dx = (T *)a.dx + offset;
-    Channels<N, is_short<T>(), A> ch;
+    Channels<N, A> ch;
     ch.load(a, n, b, at.c0);
     A m1[N], m2[N];
     int group[N];
@@ -1096,8 +1102,8 @@ template <typename T, int R, bool WRAPPED> static int launch_resident(const tode
     typedef typename Wide<T>::type A;
     const NormShape &n = p.n;
     const int groups = n.chunk / n.width, waves = p.threads / 64;
-    const size_t bytes = ((size_t)p.threads * Raw<T>::N + (groups > waves ? groups : waves) + 2 * groups) * sizeof(A);
-    static_assert((NORM_RESIDENT_THREADS + 3 * NORM_ROW_VECTORS) * Raw<T>::N * sizeof(A) <= 64 * 1024, "what a launch may have without asking");
+    const size_t bytes = ((size_t)p.threads * Raw<T>::N + 2 * groups) * sizeof(A) + (groups > waves ? groups : waves) * sizeof(double);
+    static_assert(((NORM_RESIDENT_THREADS + 2 * NORM_ROW_VECTORS) * sizeof(A) + NORM_ROW_VECTORS * sizeof(double)) * Raw<T>::N <= 64 * 1024, "what a launch may have without asking");
     hipLaunchKernelGGL((norm_resident_kernel<T, R, WRAPPED>), grid_line(p.blocks), dim3(p.threads), bytes, s, a, n);
     return check_hip(hipGetLastError(), "tode_group_norm launch");
 }
