@@ -318,3 +318,35 @@ def test_16_bit_groups_without_spread(shape, dtype, value):
     assert not dw.any()
     with torch.no_grad():
         assert torch.equal(to.group_norm(x, G, weight, bias), y)
+
+
+def activated(kind, z, grad=None):
+    """act(z), and grad * act'(z), by way of the shift of samples whose weight is zero: z reaches the activation as it is."""
+    shift = z.detach()[:, None].requires_grad_()
+    x = torch.arange(4.0, device="cuda", dtype=z.dtype)[None, :, None].expand(z.shape[0], 4, 1)
+    y = to.group_norm(x, 1, torch.zeros(1, dtype=z.dtype, device="cuda"), shift=shift, activation=kind)
+    if grad is None:
+        return y[:, 0, 0].detach()
+    cotangent = torch.zeros_like(y)
+    cotangent[:, 0, 0] = grad
+    return y[:, 0, 0].detach(), torch.autograd.grad(y, shift, cotangent)[0][:, 0]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_gelu_over_its_range(dtype):
+    """To the rounding of the result and, in float32, of the steps before it, in units of 2^-24 of the value.  The power's argument z^2 / (2 ln 2) is
+    rounded three times (the square, the constant, their product), each of which is z^2 / 2 units of the power: 3 / 2 z^2.  The reciprocal t is off by a
+    unit in the last place, which is 2, and the ratio of tail and density changes 3.2 times as fast as t at |z| = 1 and less beyond: 6.4; the power itself
+    2, the last of the polynomial's products and sums 3, three products 3: below 16."""
+    dtype = DTYPES[dtype]
+    z = torch.cat([torch.linspace(-13, 13, 400_001, dtype=torch.float64), torch.linspace(-1.01, 1.01, 200_001, dtype=torch.float64)]).to(dtype).cuda()
+    y, slope = activated("gelu", z, torch.ones_like(z))
+    want, derivative = field_oracle.activation("gelu", z.double())
+    steps = torch.finfo(dtype).eps / 2 + (2.0**-24 * (16 + 1.5 * z.double() ** 2) if dtype == torch.float32 else 2.0**-16)
+    least = 2.0**-25 if dtype == torch.float16 else 2.0**-126
+    d = (y.double() - want).abs() - (steps * want.abs() + least)
+    assert (d <= 0).all(), (z[d.argmax()], y[d.argmax()], want[d.argmax()])
+    # (the derivative is a sum of two: both are rounded)
+    terms = (want / z.double()).nan_to_num(0.5).abs() + (z.double() * torch.exp(-0.5 * z.double() ** 2) * 0.3989422804014327).abs()
+    d = (slope.double() - derivative).abs() - (steps * (terms + derivative.abs()) + least)
+    assert (d <= 0).all(), (z[d.argmax()], slope[d.argmax()], derivative[d.argmax()])

@@ -63,18 +63,32 @@ template <bool SHORT> __device__ __forceinline__ float tangent(float z) {
 }
 template <bool SHORT> __device__ __forceinline__ double tangent(double z) { return tanh(z); }
 
-// The normal distribution's function and density times sqrt(2 pi).  float32: Abramowitz and Stegun's 7.1.26, off by 7.5e-8 at most, with
-// one power and one reciprocal (erfcf takes five times as long, more than the memory needs).
-__device__ __forceinline__ void normal(float z, float &below, float &density) {
-    const float x = fabsf(z);
-    density = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170368f);
-    const float t = __builtin_amdgcn_rcpf(fmaf(x, 0.3275911f * 0.70710678118654752440f, 1.0f));
-    float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-    p = fmaf(p, t, 0.5f * 1.421413741f), p = fmaf(p, t, 0.5f * -0.284496736f), p = fmaf(p, t, 0.5f * 0.254829592f);
+// The normal distribution's function and density times sqrt(2 pi).  The tail is density times a polynomial in t = 1 / (1 + c |z|): its ratio to
+// the density falls slowly and is smooth in t.  Coefficients by weighted least squares to the smallest relative error for |z| < 14, where the
+// density ends: 6e-6 for 16 bits, 2e-8 for float32, whose |z| < 1 take an odd polynomial about 1/2 instead (4e-8 of it; differences from 1 would
+// double the error).  One power and one reciprocal; erfcf takes several times as long (512 float32 samples of 64 x 64 x 16: 76 us; 66 with five
+// coefficients for everything, which were off by 7e-8 of 1 and by a tenth of a per cent at -4; 37 float16 ones of 45 x 53 x 120: 30).
+template <bool SHORT> __device__ __forceinline__ void normal(float z, float &below, float &density) {
+    const float x = fabsf(z), s = z * z;
+    density = __builtin_amdgcn_exp2f(s * -0.72134752044448170368f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(x, SHORT ? 0.3125f : 0.2625f, 1.0f));
+    float p;
+    if (SHORT) {
+        p = fmaf(-0.0720064332f, t, 0.169261103f), p = fmaf(p, t, 0.0257095609f), p = fmaf(p, t, 0.129970966f);
+        p = fmaf(p, t, 0.122265234f), p = fmaf(p, t, 0.124796638f);
+    } else {
+        p = fmaf(0.0306574329f, t, -0.148385007f), p = fmaf(p, t, 0.233887704f), p = fmaf(p, t, -0.132396963f), p = fmaf(p, t, 0.148453724f);
+        p = fmaf(p, t, 0.0561404901f), p = fmaf(p, t, 0.102743951f), p = fmaf(p, t, 0.104149397f), p = fmaf(p, t, 0.104749262f);
+    }
     p *= t * density;
     below = z < 0 ? p : 1.0f - p;
+    if (!SHORT) {
+        float q = fmaf(9.42358652e-5f, s, -1.16935511e-3f);
+        q = fmaf(q, s, 9.96719793e-3f), q = fmaf(q, s, -6.6489583e-2f), q = fmaf(q, s, 0.398942264f);
+        below = x < 1.0f ? fmaf(q, z, 0.5f) : below;
+    }
 }
-__device__ __forceinline__ void normal(double z, double &below, double &density) {
+template <bool SHORT> __device__ __forceinline__ void normal(double z, double &below, double &density) {
     below = 0.5 * erfc(-0.70710678118654752440 * z), density = exp(-0.5 * z * z);
 }
 
@@ -86,7 +100,7 @@ template <int N, bool SHORT, typename A> __device__ __forceinline__ void activat
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             A below, density;
-            normal(z[i], below, density);
+            normal<SHORT>(z[i], below, density);
             z[i] *= below;
         }
     } else if (act == TODE_ACT_TANH) {
@@ -110,7 +124,7 @@ template <int N, bool SHORT, typename A> __device__ __forceinline__ void activat
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             A below, density;
-            normal(z[i], below, density);
+            normal<SHORT>(z[i], below, density);
             h[i] *= fma(z[i] * (A)0.398942280401432678, density, below);
         }
     } else if (act == TODE_ACT_TANH) {
