@@ -350,3 +350,24 @@ def test_gelu_over_its_range(dtype):
     terms = (want / z.double()).nan_to_num(0.5).abs() + (z.double() * torch.exp(-0.5 * z.double() ** 2) * 0.3989422804014327).abs()
     d = (slope.double() - derivative).abs() - (steps * (terms + derivative.abs()) + least)
     assert (d <= 0).all(), (z[d.argmax()], slope[d.argmax()], derivative[d.argmax()])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_activations_of_very_large_values(dtype, kind):
+    """Up to the largest numbers, and of infinity where the limit is one."""
+    dtype = DTYPES[dtype]
+    most = torch.finfo(dtype).max
+    sizes = [v for v in (20.0, 87.0, 88.5, 90.0, 104.0, 130.0, 700.0, 1000.0, 6e4, 1e20, 1e30, 2.3e38, 2.4e38, 3.3e38, 1e300) if v < most] + [most]
+    z = torch.tensor(sizes + [-v for v in sizes], dtype=torch.float64).to(dtype).cuda()
+    y, slope = activated(kind, z, torch.ones_like(z))
+    want, derivative = field_oracle.activation(kind, z.double())
+    # (values that underflow count as zero; 128 units and one for each unit of |z|, of which the power's argument has as many as it is large)
+    tolerance = torch.finfo(dtype).eps * (129 + z.double().abs().clamp(max=1000))
+    for got, value in ((y, want), (slope, derivative)):
+        d = (got.double() - value).abs()
+        assert ((d <= tolerance * value.abs() + 1e-36 + (2.0**-24 if dtype == torch.float16 else 0)) | (got.double() == value)).all(), (z[d.argmax()], got, value)
+    infinite = torch.tensor([float("inf")], dtype=dtype, device="cuda")
+    assert activated(kind, infinite).item() == (1.0 if kind == "tanh" else float("inf"))
+    assert activated(kind, -infinite).item() in {None: {-float("inf")}, "tanh": {-1.0}, "relu": {0.0}}.get(kind, set()) or kind in ("silu", "gelu")
+    assert activated(kind, torch.full_like(infinite, float("nan"))).isnan().all()

@@ -44,14 +44,13 @@ template <typename A> __device__ __forceinline__ void set_param(void *p, int dty
 template <typename T> constexpr bool is_short() { return sizeof(T) == 2; }
 
 // 1 / (1 + exp(-z)).  The hardware's power of two and reciprocal are off by one unit each; the product z log2(e) has an error that grows
-// with |z|, which float32 results carry along as `lo` (2^(hi + lo)).  (Beyond 87 they are below 2e-38 instead of a denormal.)
+// with |z|, which float32 results carry along as `lo` (2^(hi + lo)).  Where the power ends at 0 or infinity, z may be anything: it is cut off beyond
+// that, so that neither hi nor lo overflows.
 template <bool SHORT> __device__ __forceinline__ float sigmoid(float z) {
     constexpr float L = 1.44269502162933349609375f;
     if (SHORT) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -L));
-    const float t = fminf(-z, 87.0f), hi = t * L, lo = fmaf(t, L, -hi) + t * 1.9259629911266174e-8f;
-    float e = __builtin_amdgcn_exp2f(hi);
-    e = fmaf(e * lo, 0.693147180559945286f, e);
-    return __builtin_amdgcn_rcpf(1.0f + e);
+    const float t = __builtin_amdgcn_fmed3f(-z, -128.0f, 128.0f), hi = t * L, lo = fmaf(t, L, -hi) + t * 1.9259629911266174e-8f;
+    return __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(hi), fmaf(lo, 0.693147180559945286f, 1.0f), 1.0f));
 }
 template <bool SHORT> __device__ __forceinline__ double sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
 
