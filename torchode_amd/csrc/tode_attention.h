@@ -315,6 +315,11 @@ inline long long placed(const tode_cross_attention_args &a, int tiles) {
 // host side
 // ------------------------------------------------------------------------------------------
 
+// More than 64 KiB of LDS is to be asked for, kernel by kernel.
+inline int allow_lds(const void *kernel, int bytes) {
+    return bytes > 64 * 1024 ? check_hip(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute") : TODE_OK;
+}
+
 // The sources are compiled once for each element type.
 #define TODE_ATT_JOIN_(name, suffix) name##_##suffix
 #define TODE_ATT_JOIN(name, suffix) TODE_ATT_JOIN_(name, suffix)

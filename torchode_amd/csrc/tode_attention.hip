@@ -660,8 +660,7 @@ template <typename T, int DP, int WC, int WS> static int launch(const tode_cross
     constexpr int tile_bytes = WS * 2 * L::VALUES * (int)sizeof(T), join_bytes = WS > 1 ? WS * (L::NT * 16 + 2) * 64 * 4 : 0;
     constexpr int bytes = tile_bytes > join_bytes ? tile_bytes : join_bytes;
     static_assert(bytes <= 160 * 1024, "LDS");
-    if (bytes > 64 * 1024)
-        if (int rc = check_hip(hipFuncSetAttribute((const void *)attention_kernel<T, DP, WC, WS>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute")) return rc;
+    if (int rc = allow_lds((const void *)attention_kernel<T, DP, WC, WS>, bytes)) return rc;
     hipLaunchKernelGGL((attention_kernel<T, DP, WC, WS>), grid_line(placed(a, p.tiles * p.splits)), dim3(64 * WC * WS), bytes, s, a, p.tiles, p.splits, (float *)a.workspace);
     if (p.splits > 1) {
         const long long rows = p.groups * a.queries * (a.heads / a.kv_heads);
@@ -674,8 +673,7 @@ template <typename T, int DP, int CT> static int launch_tiles(const tode_cross_a
     typedef Tile<T, DP> L;
     constexpr int bytes = 4 * (DP > 128 ? 32 : 64) * L::STRIDE * (int)sizeof(T);
     static_assert(bytes <= 160 * 1024, "LDS");
-    if (bytes > 64 * 1024)
-        if (int rc = check_hip(hipFuncSetAttribute((const void *)attention_tiles_kernel<T, DP, CT>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute")) return rc;
+    if (int rc = allow_lds((const void *)attention_tiles_kernel<T, DP, CT>, bytes)) return rc;
     hipLaunchKernelGGL((attention_tiles_kernel<T, DP, CT>), grid_line(placed(a, p.tiles * p.splits)), dim3(256), bytes, s, a, p.tiles, p.splits, (float *)a.workspace);
     if (p.splits > 1) {
         const long long rows = p.groups * a.queries * (a.heads / a.kv_heads);
@@ -691,8 +689,7 @@ template <typename T, int DP, int SUBS> static int launch_short(const tode_cross
     if constexpr (bytes > 160 * 1024)
         return fail(TODE_E_UNSUPPORTED, "head_dim %d", a.head_dim);
     else {
-        if (bytes > 64 * 1024)
-            if (int rc = check_hip(hipFuncSetAttribute((const void *)attention_short_kernel<T, DP, SUBS, WAVES>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute")) return rc;
+        if (int rc = allow_lds((const void *)attention_short_kernel<T, DP, SUBS, WAVES>, bytes)) return rc;
         const long long rows = a.queries * (a.heads / a.kv_heads), row_tiles = (rows + 31) / 32;
         // a wavefront takes two tiles of rows or more where there are a thousand workgroups without it
         const long long most = (row_tiles + WAVES - 1) / WAVES, wanted = (1024 + p.groups - 1) / p.groups;

@@ -449,16 +449,20 @@ static BackwardPlan plan_backward(const tode_cross_attention_args &a) {
 
 template <typename T, int DP, int WC, int WS> static int launch_dq(const tode_cross_attention_args &a, const BackwardPlan &p, hipStream_t s) {
     typedef Tile<T, DP> L;
-    constexpr int tile_bytes = WS * 2 * L::VALUES * (int)sizeof(T), join_bytes = WS > 1 ? WS * L::NT * 16 * 64 * 4 : 0;
-    constexpr int bytes = tile_bytes > join_bytes ? tile_bytes : join_bytes;
-    static_assert(bytes <= 160 * 1024, "LDS");
-    if (bytes > 64 * 1024)
-        if (int rc = check_hip(hipFuncSetAttribute((const void *)attention_dq_kernel<T, DP, WC, WS>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute")) return rc;
     float *const sums = (float *)a.workspace, *const partial = (float *)((char *)a.workspace + p.sums);
-    if constexpr (sizeof(T) == 2 && WC == 4)
-        hipLaunchKernelGGL((attention_dq_tiles_kernel<T, DP>), grid_line(placed(a, p.row_tiles * p.row_splits)), dim3(256), 4 * L::VALUES * sizeof(T), s, a, p.row_tiles, p.row_splits, sums, partial);
-    else
-        hipLaunchKernelGGL((attention_dq_kernel<T, DP, WC, WS>), grid_line(placed(a, p.row_tiles * p.row_splits)), dim3(64 * WC * WS), bytes, s, a, p.row_tiles, p.row_splits, sums, partial);
+    const dim3 grid = grid_line(placed(a, p.row_tiles * p.row_splits));
+    if constexpr (sizeof(T) == 2 && WC == 4) {
+        constexpr int bytes = 4 * L::VALUES * (int)sizeof(T);
+        static_assert(bytes <= 160 * 1024, "LDS");
+        if (int rc = allow_lds((const void *)attention_dq_tiles_kernel<T, DP>, bytes)) return rc;
+        hipLaunchKernelGGL((attention_dq_tiles_kernel<T, DP>), grid, dim3(256), bytes, s, a, p.row_tiles, p.row_splits, sums, partial);
+    } else {
+        constexpr int tile_bytes = WS * 2 * L::VALUES * (int)sizeof(T), join_bytes = WS > 1 ? WS * L::NT * 16 * 64 * 4 : 0;
+        constexpr int bytes = tile_bytes > join_bytes ? tile_bytes : join_bytes;
+        static_assert(bytes <= 160 * 1024, "LDS");
+        if (int rc = allow_lds((const void *)attention_dq_kernel<T, DP, WC, WS>, bytes)) return rc;
+        hipLaunchKernelGGL((attention_dq_kernel<T, DP, WC, WS>), grid, dim3(64 * WC * WS), bytes, s, a, p.row_tiles, p.row_splits, sums, partial);
+    }
     if (p.row_splits > 1) {
         const long long n = a.batch * a.queries * a.heads * a.head_dim;
         hipLaunchKernelGGL((attention_add_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, n, p.row_splits, n, (const float *)partial, (float)a.scale, (T *)a.dq);
@@ -468,20 +472,21 @@ template <typename T, int DP, int WC, int WS> static int launch_dq(const tode_cr
 
 template <typename T, int DP, int WC, int WS> static int launch_dkv(const tode_cross_attention_args &a, const BackwardPlan &p, hipStream_t s) {
     typedef Tile<T, DP> L;
-    constexpr int tile_bytes = WS * (2 * L::VALUES * (int)sizeof(T) + 64 * 4), join_bytes = WS > 1 ? WS * L::NT * 16 * 64 * 4 : 0;
-    constexpr int bytes = tile_bytes > join_bytes ? tile_bytes : join_bytes;
-    static_assert(bytes <= 160 * 1024, "LDS");
-    if (bytes > 64 * 1024)
-        if (int rc = check_hip(hipFuncSetAttribute((const void *)attention_dkv_kernel<T, DP, WC, WS>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "hipFuncSetAttribute")) return rc;
     float *const sums = (float *)a.workspace, *const partial = (float *)((char *)a.workspace + p.sums);
     if constexpr (sizeof(T) == 2 && WC == 4 && DP <= 128) {
-        constexpr int tiles_bytes = 8 * L::VALUES * (int)sizeof(T) + 1024;
-        if (tiles_bytes > 64 * 1024)
-            if (int rc = check_hip(hipFuncSetAttribute((const void *)attention_dkv_tiles_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, tiles_bytes), "hipFuncSetAttribute")) return rc;
-        hipLaunchKernelGGL((attention_dkv_tiles_kernel<T, DP>), grid_line(placed(a, 2 * p.key_tiles * p.key_splits)), dim3(256), tiles_bytes, s, a, p.key_tiles, p.key_splits,
-                           (const float *)sums, partial);
-    } else
-        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, WC, WS>), grid_line(placed(a, p.key_tiles * p.key_splits)), dim3(64 * WC * WS), bytes, s, a, p.key_tiles, p.key_splits, (const float *)sums, partial);
+        constexpr int bytes = 8 * L::VALUES * (int)sizeof(T) + 1024;
+        static_assert(bytes <= 160 * 1024, "LDS");
+        if (int rc = allow_lds((const void *)attention_dkv_tiles_kernel<T, DP>, bytes)) return rc;
+        hipLaunchKernelGGL((attention_dkv_tiles_kernel<T, DP>), grid_line(placed(a, 2 * p.key_tiles * p.key_splits)), dim3(256), bytes, s, a, p.key_tiles, p.key_splits, (const float *)sums,
+                           partial);
+    } else {
+        constexpr int tile_bytes = WS * (2 * L::VALUES * (int)sizeof(T) + 64 * 4), join_bytes = WS > 1 ? WS * L::NT * 16 * 64 * 4 : 0;
+        constexpr int bytes = tile_bytes > join_bytes ? tile_bytes : join_bytes;
+        static_assert(bytes <= 160 * 1024, "LDS");
+        if (int rc = allow_lds((const void *)attention_dkv_kernel<T, DP, WC, WS>, bytes)) return rc;
+        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, WC, WS>), grid_line(placed(a, p.key_tiles * p.key_splits)), dim3(64 * WC * WS), bytes, s, a, p.key_tiles, p.key_splits, (const float *)sums,
+                           partial);
+    }
     if (p.key_splits > 1) {
         const long long n = a.batch * a.keys * a.kv_heads * a.head_dim;
         hipLaunchKernelGGL((attention_add_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, n, p.key_splits, 2 * n, (const float *)partial, (float)a.scale, (T *)a.dk);
