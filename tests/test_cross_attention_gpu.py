@@ -425,3 +425,39 @@ def test_more_workgroups_than_a_grid_has_in_a_row(batch, training):
     for first in range(0, batch, step):
         part = run({k: v.detach()[first : first + step].requires_grad_(training) for k, v in t.items()}, grad[first : first + step])
         assert all(torch.equal(a[first : first + step], b) for a, b in zip(whole, part))
+
+
+# Sizes that take each form of many samples: float32 with 512 groups of 128 rows and more (four wavefronts on tiles that they share, and up to 128 keys in
+# LDS), single tokens with more of them than share keys between wavefronts, and every number of 32 keys that stays in LDS.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(
+    "shape",
+    [
+        (256, 40, 70, 2, 2, 32),
+        (256, 140, 100, 2, 2, 64),
+        (513, 33, 128, 1, 1, 64),
+        (256, 20, 70, 4, 2, 32),
+        (256, 40, 129, 2, 2, 32),
+        (256, 50, 300, 2, 2, 64),
+        (130, 70, 129, 4, 4, 80),
+        (128, 130, 300, 4, 4, 128),
+        (70, 200, 300, 9, 9, 20),
+        (2, 300, 60, 2, 1, 128),
+        (2, 300, 70, 2, 1, 128),
+        (2, 300, 128, 2, 2, 32),
+        (2, 200, 500, 2, 2, 96),
+        (8200, 1, 200, 1, 1, 32),
+        (2100, 2, 40, 4, 4, 16),
+        (1100, 3, 33, 8, 8, 8),
+        (300, 7, 700, 2, 2, 40),
+    ],
+    ids=ids,
+)
+def test_forms_of_many_samples(shape, dtype):
+    check(*made(shape, DTYPES[dtype], lengths="ragged", holes=0.2, seed=sum(shape)), DTYPES[dtype])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_forms_of_many_samples_without_a_mask(dtype):
+    """(and without lengths: tiles of which every key may be looked at take a shorter way)"""
+    check(*made((256, 140, 320, 2, 2, 64), DTYPES[dtype], seed=35), DTYPES[dtype])

@@ -371,3 +371,44 @@ def test_activations_of_very_large_values(dtype, kind):
     assert activated(kind, infinite).item() == (1.0 if kind == "tanh" else float("inf"))
     assert activated(kind, -infinite).item() in {None: {-float("inf")}, "tanh": {-1.0}, "relu": {0.0}}.get(kind, set()) or kind in ("silu", "gelu")
     assert activated(kind, torch.full_like(infinite, float("nan"))).isnan().all()
+
+
+# Parts of a sample that take 16 and 32 vectors a thread, with rows of whole vectors and of several positions: 128 workgroups or more of 64 KiB and more.
+@pytest.mark.parametrize(
+    "dtype,shape",
+    [
+        ("f32", (130, (64, 60), 8, 2)),
+        ("f32", (130, (64, 64), 16, 4)),
+        ("f32", (130, (72, 64), 16, 4)),
+        ("f32", (130, (4501,), 6, 2)),
+        ("f64", (130, (64, 60), 4, 2)),
+        ("f64", (130, (90, 70), 4, 2)),
+        ("f64", (130, (4501,), 3, 1)),
+        ("bf16", (130, (60, 50), 16, 2)),
+        ("bf16", (130, (90, 70), 16, 2)),
+        ("bf16", (64, (40, 40), 320, 32)),
+        ("f16", (130, (90, 70), 16, 2)),
+        ("f16", (130, (4501,), 12, 3)),
+    ],
+    ids=lambda v: v if isinstance(v, str) else "x".join(map(str, (v[0], *v[1], v[2]))),
+)
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+def test_parts_of_many_vectors(dtype, shape, kind):
+    t, dy = made(shape, DTYPES[dtype], params=DTYPES[dtype], modulated=True, seed=22)
+    check(shape, DTYPES[dtype], kind, t, dy)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, (s[0], *s[1], s[2]))) + f"g{s[3]}")
+def test_values_without_a_graph(shape, dtype):
+    """No statistics are asked for there: to the last bit what a call with them gives, and that by its definition."""
+    i = SHAPES.index(shape)
+    t, _ = made(shape, DTYPES[dtype], params=DTYPES[dtype], modulated=i % 2 == 0, seed=i)
+    kind, names = KINDS[i % 5], ("weight", "bias", "scale", "shift")
+    call = lambda x: to.group_norm(x, shape[3], t["weight"], t["bias"], scale=t.get("scale"), shift=t.get("shift"), activation=kind)
+    with torch.no_grad():
+        y = call(t["x"])
+    graph = call(t["x"].clone().requires_grad_())
+    assert graph.requires_grad and not y.requires_grad and torch.equal(y, graph)
+    want = field_oracle.group_norm(DTYPES[dtype], t["x"].double(), shape[3], *(t[k].double() if k in t else None for k in names), kind, 1e-5)
+    field_oracle.assert_close(y, *want["y"], "y", dtype=DTYPES[dtype])
