@@ -445,15 +445,20 @@ def test_more_workgroups_than_a_grid_has_in_a_row(batch, training):
         (2, 300, 60, 2, 1, 128),
         (2, 300, 70, 2, 1, 128),
         (2, 300, 128, 2, 2, 32),
+        (2, 300, 120, 2, 1, 128),
+        (513, 40, 90, 1, 1, 64),
         (2, 200, 500, 2, 2, 96),
         (8200, 1, 200, 1, 1, 32),
         (2100, 2, 40, 4, 4, 16),
         (1100, 3, 33, 8, 8, 8),
         (300, 7, 700, 2, 2, 40),
+        (3, 40, 20, 2, 1, 200),
     ],
     ids=ids,
 )
 def test_forms_of_many_samples(shape, dtype):
+    if dtype == "f32" and shape[5] > 128:
+        pytest.skip("float32 heads have up to 128 values")
     check(*made(shape, DTYPES[dtype], lengths="ragged", holes=0.2, seed=sum(shape)), DTYPES[dtype])
 
 

@@ -388,7 +388,9 @@ def test_activations_of_very_large_values(dtype, kind):
         ("bf16", (130, (90, 70), 16, 2)),
         ("bf16", (64, (40, 40), 320, 32)),
         ("f16", (130, (90, 70), 16, 2)),
+        ("f16", (130, (60, 50), 16, 2)),
         ("f16", (130, (4501,), 12, 3)),
+        ("bf16", (130, (4501,), 12, 3)),
     ],
     ids=lambda v: v if isinstance(v, str) else "x".join(map(str, (v[0], *v[1], v[2]))),
 )
@@ -412,3 +414,14 @@ def test_values_without_a_graph(shape, dtype):
     assert graph.requires_grad and not y.requires_grad and torch.equal(y, graph)
     want = field_oracle.group_norm(DTYPES[dtype], t["x"].double(), shape[3], *(t[k].double() if k in t else None for k in names), kind, 1e-5)
     field_oracle.assert_close(y, *want["y"], "y", dtype=DTYPES[dtype])
+
+
+@pytest.mark.parametrize("positions", [180, 400, 900, 2000])
+@pytest.mark.parametrize("wrapped", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_parts_of_few_vectors(dtype, wrapped, positions):
+    """One to eight vectors a thread: two or three of them in a row of one or two positions."""
+    vector = 128 // torch.finfo(DTYPES[dtype]).bits
+    shape = (9, (positions + 1,), vector * 3 // 2 if wrapped else 2 * vector, 3 if wrapped else 2)
+    t, dy = made(shape, DTYPES[dtype], params=DTYPES[dtype], modulated=True, seed=positions)
+    check(shape, DTYPES[dtype], KINDS[positions % 5], t, dy)

@@ -1155,7 +1155,7 @@ template <typename T> static int forward_resident(const tode_group_norm_args &a,
         case 4: TODE_NORM_R(launch_resident, 4);
         case 8: TODE_NORM_R(launch_resident, 8);
         case 16: TODE_NORM_R(launch_resident, 16);
-        default: TODE_NORM_R(launch_resident, 32);
+        default: return launch_resident<T, 32, false>(a, p, s);  // (rows of several positions take half as many)
     }
 }
 template <typename T> static int backward_resident(const tode_group_norm_args &a, const ResidentPlan &p, hipStream_t s) {
@@ -1163,7 +1163,7 @@ template <typename T> static int backward_resident(const tode_group_norm_args &a
         case 1: TODE_NORM_R(launch_resident_backward, 1);
         case 2: TODE_NORM_R(launch_resident_backward, 2);
         case 4: TODE_NORM_R(launch_resident_backward, 4);
-        default: TODE_NORM_R(launch_resident_backward, 8);
+        default: return launch_resident_backward<T, 8, false>(a, p, s);
     }
 }
 #undef TODE_NORM_R
