@@ -466,3 +466,19 @@ def test_forms_of_many_samples(shape, dtype):
 def test_forms_of_many_samples_without_a_mask(dtype):
     """(and without lengths: tiles of which every key may be looked at take a shorter way)"""
     check(*made((256, 140, 320, 2, 2, 64), DTYPES[dtype], seed=35), DTYPES[dtype])
+
+
+def test_tangents_are_refused():
+    t, _, grad = made((2, 3, 5, 2, 1, 8), torch.float32)
+    q = t["q"].requires_grad_()
+    out = to.cross_attention(**t)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(out, q, torch.autograd.forward_ad.make_dual(grad, grad))
+
+    def derivative(v):
+        return torch.func.jvp(lambda v: to.cross_attention(v, t["k"], t["v"]), (v,), (torch.ones_like(v),))
+
+    for f in (derivative, torch.compile(derivative, backend="eager")):
+        with pytest.raises(NotImplementedError, match="jvp|forward-mode"):
+            f(q.detach())

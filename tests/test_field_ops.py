@@ -129,3 +129,21 @@ def test_c_entry_of_cross_attention_refuses_negative_strides(name):
             assert lib.tode_cross_attention_workspace_bytes(C.byref(args), 0) == _lib.E_INVALID
             assert lib.tode_cross_attention(C.byref(args), None) == _lib.E_INVALID and b"negative" in lib.tode_last_error()
     assert lib.tode_cross_attention(C.byref(attention_args(mask_stride=-3)), None) == _lib.E_INVALID and b"negative" in lib.tode_last_error()
+
+
+# The operators and their differentiable arguments, small and on the CPU: what is refused there is refused ahead of the device.
+CALLS = {
+    "group_norm": (dict(x=Z(2, 3, 4), weight=Z(4), bias=Z(4), scale=Z(2, 4), shift=Z(2, 4)), lambda t: to.group_norm(t["x"], 2, t["weight"], t["bias"], scale=t["scale"], shift=t["shift"])),
+    "cross_attention": (dict(q=Q, k=K, v=K.clone()), lambda t: to.cross_attention(**t)),
+}
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("name,argument", [(n, a) for n, (tensors, _) in CALLS.items() for a in tensors])
+def test_tangents_are_refused(name, argument, requires_grad):
+    tensors, call = CALLS[name]
+    t = {k: v.clone().requires_grad_(requires_grad) for k, v in tensors.items()}
+    with torch.autograd.forward_ad.dual_level():
+        t[argument] = torch.autograd.forward_ad.make_dual(t[argument], torch.ones_like(t[argument]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(t)

@@ -425,3 +425,19 @@ def test_parts_of_few_vectors(dtype, wrapped, positions):
     shape = (9, (positions + 1,), vector * 3 // 2 if wrapped else 2 * vector, 3 if wrapped else 2)
     t, dy = made(shape, DTYPES[dtype], params=DTYPES[dtype], modulated=True, seed=positions)
     check(shape, DTYPES[dtype], KINDS[positions % 5], t, dy)
+
+
+def test_tangents_are_refused():
+    x = torch.randn(2, 5, 4, device="cuda", requires_grad=True)
+    y = to.group_norm(x, 2)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, x, dual)
+
+    def derivative(v):
+        return torch.func.jvp(lambda v: to.group_norm(v, 2), (v,), (torch.ones_like(v),))
+
+    for f in (derivative, torch.compile(derivative, backend="eager")):
+        with pytest.raises(NotImplementedError, match="jvp|forward-mode"):
+            f(x.detach())

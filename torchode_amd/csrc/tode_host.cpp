@@ -261,6 +261,10 @@ bool recorded(std::initializer_list<const Tensor *> tensors) {
         if (t->defined() && t->requires_grad()) return true;
     return false;
 }
+// There is no forward-mode derivative: a tangent (of torch.autograd.forward_ad; torch.func's has its own refusal) would be lost without a word.
+void without_tangent(const char *operation, std::initializer_list<const Tensor *> tensors) {
+    for (const Tensor *t : tensors) TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), operation, " has no forward-mode derivative");
+}
 // Gradients as a backward pass returns them: where a graph of it is asked for, results of a node that says that there is none.
 variable_list once(variable_list gradients, const char *message, const variable_list &inputs, const Tensor &cotangent) {
     if (!c10::GradMode::is_enabled()) return gradients;
@@ -302,6 +306,7 @@ struct NormCall {
         bool affine = false, modulation = false;
         weight = parameter(weight_, "weight", true, a.affine_dtype, affine), bias = parameter(bias_, "bias", true, a.affine_dtype, affine);
         scale = parameter(scale_, "scale", false, a.modulation_dtype, modulation), shift = parameter(shift_, "shift", false, a.modulation_dtype, modulation);
+        without_tangent("group_norm", {&x, &weight_, &bias_, &scale_, &shift_});
         TORCH_CHECK(x.is_cuda(), NEEDS_GPU, x.device(), "'. There is no CPU implementation to fall back to.");
         x = x.contiguous();
         a.n_groups = (int32_t)G, a.channels = (int32_t)C, a.batch = B, a.positions = 1;
@@ -330,6 +335,7 @@ struct NormCall {
     // of x, weight, bias, scale, shift: undefined where bit i of `want` is not set
     variable_list backward(const Tensor &dy_, const Tensor &mean, const Tensor &rstd, int64_t want) {
         TORCH_CHECK_VALUE(dy_.sizes() == x.sizes() && dy_.scalar_type() == x.scalar_type() && dy_.device() == x.device(), "group_norm: the cotangent must be like x");
+        without_tangent("group_norm's gradient", {&dy_});
         for (const Tensor *t : {&mean, &rstd})
             TORCH_CHECK_VALUE(t->dim() == 2 && t->size(0) == a.batch && t->size(1) == a.n_groups && t->is_contiguous() && t->scalar_type() == statistics && t->device() == x.device(), "group_norm: mean and rstd must be [batch, groups] as the forward pass returned them");
         const Tensor dy = dy_.contiguous();
@@ -429,6 +435,7 @@ struct AttentionCall {
         TORCH_CHECK_VALUE(std::isfinite(a.scale), "cross_attention: scale must be finite, got ", a.scale);
         for (const Tensor *t : {&k, &v, &lengths, &mask})
             TORCH_CHECK_VALUE(!t->defined() || t->device() == q.device(), "cross_attention: a tensor is on ", t->device(), ", q on ", q.device());
+        without_tangent("cross_attention", {&q, &k, &v});
         TORCH_CHECK(q.is_cuda(), NEEDS_GPU, q.device(), "'. There is no CPU implementation to fall back to.");
         q = rows(q, a.q_strides), k = rows(k, a.k_strides), v = rows(v, a.v_strides);
         if (lengths.defined()) lengths = lengths.contiguous();
@@ -461,6 +468,7 @@ struct AttentionCall {
         for (const Tensor *t : {&grad_, &out})
             TORCH_CHECK_VALUE(t->sizes() == q.sizes() && t->scalar_type() == q.scalar_type() && t->device() == q.device(), "cross_attention: the output and its cotangent must be like q");
         TORCH_CHECK_VALUE(low.is_contiguous() && low.scalar_type() == q.scalar_type() && low.device() == q.device() && (a.dtype == TODE_F32 ? low.numel() == 0 : low.sizes() == q.sizes()) && out.is_contiguous() && lse.is_contiguous() && lse.sizes() == q.sizes().slice(0, 3) && lse.scalar_type() == at::kFloat && lse.device() == q.device(), "cross_attention: out, low and lse must be as the forward pass returned them");
+        without_tangent("cross_attention's gradient", {&grad_});
         const Tensor grad = rows(grad_, a.grad_strides);
         const c10::DeviceGuard guard(q.device());
         variable_list g(3);

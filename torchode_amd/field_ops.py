@@ -8,17 +8,24 @@ graphs of its iterations (``graph_iterations``), both backsolve adjoints (``Back
 ``vmap``: shape the state with ``y.reshape(-1, ...)`` there), ``torch.compile`` of ``f``.  Samples stay independent of each other, as
 the solver takes them to be.
 
-Neither is differentiable twice.  The reference leaves ``f`` to the user (terms.py:13-19).
+Neither is differentiable twice or in forward mode: both are refused (``NotImplementedError``, ``RuntimeError`` from PyTorch).  The reference leaves ``f`` to the user (terms.py:13-19).
 """
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
 # A call inside torch.func.vmap, vjp, ... hands out tensors in wrappers: those go through the autograd.Functions below, others through
 # nodes of the extension (csrc/tode_host.cpp).
 _transformed = torch._C._are_functorch_transforms_active
+
+
+def _without_tangents(name, *tensors):
+    """In a program that is being compiled (elsewhere the extension looks): PyTorch lets operators without a forward-mode derivative drop tangents."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def group_norm(
@@ -47,6 +54,7 @@ def group_norm(
     if torch.compiler.is_compiling():
         from . import ops
 
+        _without_tangents("group_norm", x, weight, bias, scale, shift)
         return ops.group_norm(x, n_groups, weight, bias, scale, shift, act, eps)
     if _transformed():
         return _GroupNorm.apply(x, weight, bias, scale, shift, n_groups, act, eps)[0]
@@ -160,6 +168,7 @@ def cross_attention(
     if torch.compiler.is_compiling():
         from . import ops
 
+        _without_tangents("cross_attention", q, k, v)
         return ops.cross_attention(q, k, v, lengths, mask, scale)
     if _transformed():
         return _CrossAttention.apply(q, k, v, lengths, mask, scale)[0]
