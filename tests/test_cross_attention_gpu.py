@@ -482,3 +482,42 @@ def test_tangents_are_refused():
     for f in (derivative, torch.compile(derivative, backend="eager")):
         with pytest.raises(NotImplementedError, match="jvp|forward-mode"):
             f(q.detach())
+
+
+@pytest.mark.parametrize("how", ["trace", "make_fx", "make_fx of gradients", "make_fx of vjp", "make_fx of vmap", "make_fx of a backward pass", "make_fx, symbolic"])
+def test_recorded_programs(how):
+    """What records a program sees the operation: its replay computes from new inputs what a call does."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    (first, dy), (other, _) = ((list(t.values()), dy) for t, _, dy in (made((3, 5, 7, 4, 2, 16), torch.bfloat16, seed=s) for s in (36, 37)))
+    lengths = torch.tensor([7, 0, 4], device="cuda")
+
+    def call(q, k, v):
+        return to.cross_attention(q, k, v, lengths=None if how in ("make_fx of vmap", "make_fx, symbolic") else lengths)
+
+    def gradients(*values):
+        leaves = [v.detach().requires_grad_() for v in values]
+        return torch.autograd.grad(call(*leaves), leaves, dy)
+
+    def pulled(*values):
+        return torch.func.vjp(call, *values)[1](dy)
+
+    def mapped(*values):
+        return torch.func.vmap(lambda *one: call(*(v[None] for v in one))[0])(*values)
+
+    f = {"make_fx of gradients": gradients, "make_fx of vjp": pulled, "make_fx of vmap": mapped}.get(how, call)
+    if how == "make_fx of a backward pass":  # (of a graph that was there before)
+        leaves = [v.clone().requires_grad_() for v in first]
+        y = call(*leaves)
+        program = make_fx(lambda g: torch.autograd.grad(y, leaves, g, retain_graph=True))(dy)
+        for got, want in zip(program(2 * dy), torch.autograd.grad(y, leaves, 2 * dy)):
+            assert torch.equal(got, want)
+        return
+    with torch.no_grad() if how == "trace" else torch.enable_grad():
+        program = torch.jit.trace(f, tuple(first)) if how == "trace" else make_fx(f, tracing_mode="symbolic" if "symbolic" in how else "real")(*first)
+    held = torch.empty(1 << 20, device="cuda").fill_(7)  # (memory that a program without its kernels would find)
+    del held
+    for values in (first, other):
+        got, want = program(*values), f(*values)
+        for a, b in zip(*((x,) if torch.is_tensor(x) else x for x in (got, want))):
+            assert torch.equal(a, b)

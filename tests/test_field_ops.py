@@ -147,3 +147,26 @@ def test_tangents_are_refused(name, argument, requires_grad):
         t[argument] = torch.autograd.forward_ad.make_dual(t[argument], torch.ones_like(t[argument]))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             call(t)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_recorded_programs_hold_the_operation(name):
+    """Whatever records a program or looks on sees an operation of the dispatcher, and not the allocation of its result."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    import torchode_amd.ops  # noqa: F401 (registers them)
+
+    tensors, call = CALLS[name]
+    operation = getattr(torch.ops.torchode_amd, name)
+    with FakeTensorMode():
+        t = {k: torch.empty(v.shape, device="cuda:0") for k, v in tensors.items()}
+        first = next(iter(t.values()))
+        out = call(t)
+        assert out.shape == first.shape and out.device == first.device
+
+        def program(*values):
+            return call(dict(zip(t, values)))
+
+        graph = make_fx(program)(*t.values()).graph
+        assert [n.target for n in graph.nodes if n.op == "call_function"][0] == operation.default, graph

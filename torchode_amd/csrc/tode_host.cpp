@@ -8,12 +8,14 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 
@@ -261,6 +263,18 @@ bool recorded(std::initializer_list<const Tensor *> tensors) {
         if (t->defined() && t->requires_grad()) return true;
     return false;
 }
+// Whether someone records what is called or looks on: torch.jit.trace, modes like those of make_fx and FakeTensorMode, tensors that dispatch to Python. They see
+// the dispatcher's operations only, so a call from here would leave the allocation of its result and not what fills it.
+bool watched(std::initializer_list<const Tensor *> tensors) {
+    if (torch::jit::tracer::isTracing() || c10::impl::dispatch_mode_enabled()) return true;
+    for (const Tensor *t : tensors)
+        if (t->defined() && t->unsafeGetTensorImpl()->is_python_dispatch()) return true;
+    return false;
+}
+PyObject *none() {
+    Py_INCREF(Py_None);
+    return Py_None;
+}
 // There is no forward-mode derivative: a tangent (of torch.autograd.forward_ad; torch.func's has its own refusal) would be lost without a word.
 void without_tangent(const char *operation, std::initializer_list<const Tensor *> tensors) {
     for (const Tensor *t : tensors) TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), operation, " has no forward-mode derivative");
@@ -272,6 +286,51 @@ variable_list once(variable_list gradients, const char *message, const variable_
     for (Tensor &t : gradients)
         if (t.defined()) torch::autograd::set_history(t, node);
     return gradients;
+}
+
+// A backward pass that something looks on at, or whose cotangent a transform of torch.func has wrapped: the functions of field_ops.py know both.
+bool beyond_here(const Tensor &cotangent) {
+    const auto keys = cotangent.unsafeGetTensorImpl()->key_set();
+    return watched({&cotangent}) || keys.has(c10::DispatchKey::FuncTorchBatched) || keys.has(c10::DispatchKey::FuncTorchGradWrapper);
+}
+struct WithGil {
+    PyGILState_STATE state = PyGILState_Ensure();
+    ~WithGil() { PyGILState_Release(state); }
+};
+struct Owned {  // a reference, or a Python error to be thrown
+    PyObject *object;
+    explicit Owned(PyObject *o) : object(o) {
+        if (o) return;
+        python_error e;
+        e.persist();
+        throw e;
+    }
+    ~Owned() { Py_DECREF(object); }
+    Owned(const Owned &) = delete;
+};
+PyObject *argument(const Tensor &t) { return t.defined() ? THPVariable_Wrap(t) : none(); }
+PyObject *argument(int64_t v) { return PyLong_FromLongLong(v); }
+PyObject *argument(double v) { return PyFloat_FromDouble(v); }
+PyObject *argument(bool v) { return PyBool_FromLong(v); }
+// torchode_amd.field_ops.<function>.apply(...), a tuple of tensors and None
+template <typename... A> variable_list applied(const char *function, const A &...of) {
+    const WithGil gil;
+    const Owned arguments(PyTuple_New(sizeof...(A)));
+    Py_ssize_t i = 0;
+    ([&] {
+        PyObject *const o = argument(of);
+        PyTuple_SET_ITEM(arguments.object, i++, o ? o : none());
+        if (!o) Owned{nullptr};
+    }(), ...);
+    const Owned module(PyImport_ImportModule("torchode_amd.field_ops")), type(PyObject_GetAttrString(module.object, function)), apply(PyObject_GetAttrString(type.object, "apply"));
+    const Owned result(PyObject_Call(apply.object, arguments.object, nullptr));
+    const Owned tuple(PySequence_Tuple(result.object));
+    variable_list tensors;
+    for (Py_ssize_t k = 0; k < PyTuple_GET_SIZE(tuple.object); ++k) {
+        PyObject *const item = PyTuple_GET_ITEM(tuple.object, k);
+        tensors.push_back(THPVariable_Check(item) ? THPVariable_Unpack(item) : Tensor());
+    }
+    return tensors;
 }
 
 // x [B, ..., C], weight and bias [C] ([B, C]: one for each sample), scale and shift [B, C]: checked, and as the kernels take them
@@ -365,26 +424,32 @@ struct NormNode : torch::autograd::Function<NormNode> {
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
         if (!grads[0].defined()) return variable_list(8);
         const variable_list saved = ctx->get_saved_variables();
+        const int64_t groups = ctx->saved_data["groups"].toInt(), activation = ctx->saved_data["activation"].toInt();
+        int64_t want = 0;
+        size_t edge = 0;
+        for (int i = 0; i < 5; ++i)
+            if (saved[i].defined()) want |= (int64_t)ctx->needs_input_grad(edge++) << i;
         variable_list gradients;
-        {
-            const at::AutoDispatchBelowADInplaceOrView below;
-            NormCall call(saved[0], saved[1], saved[2], saved[3], saved[4], ctx->saved_data["groups"].toInt(), ctx->saved_data["activation"].toInt());
-            int64_t want = 0;
-            size_t edge = 0;
-            for (int i = 0; i < 5; ++i)
-                if (saved[i].defined()) want |= (int64_t)ctx->needs_input_grad(edge++) << i;
-            gradients = call.backward(grads[0], saved[5], saved[6], want);
+        if (beyond_here(grads[0]))
+            gradients = applied("_GroupNormBackward", grads[0], saved[0], saved[5], saved[6], saved[1], saved[2], saved[3], saved[4], groups, activation, want);
+        else {
+            {
+                const at::AutoDispatchBelowADInplaceOrView below;
+                NormCall call(saved[0], saved[1], saved[2], saved[3], saved[4], groups, activation);
+                gradients = call.backward(grads[0], saved[5], saved[6], want);
+            }
+            gradients = once(std::move(gradients), "group_norm is not differentiable twice", saved, grads[0]);
         }
-        gradients = once(std::move(gradients), "group_norm is not differentiable twice", saved, grads[0]);
         gradients.resize(8);
         return gradients;
     }
 };
 
-// group_norm(x, n_groups, weight, bias, scale, shift, activation, eps) -> y
+// group_norm(x, n_groups, weight, bias, scale, shift, activation, eps) -> y, or None: to go through the dispatcher
 PyObject *group_norm_(PyObject *const *arg) {
     const Tensor &x = tensor(arg[0], "x");
     const Tensor weight = optional(arg[2], "weight"), bias = optional(arg[3], "bias"), scale = optional(arg[4], "scale"), shift = optional(arg[5], "shift");
+    if (watched({&x, &weight, &bias, &scale, &shift})) return none();
     const long long groups = integer(arg[1]), activation = integer(arg[6]);
     const double eps = number(arg[7]);
     if (recorded({&x, &weight, &bias, &scale, &shift})) return THPVariable_Wrap(NormNode::apply(x, if_there(weight), if_there(bias), if_there(scale), if_there(shift), (int64_t)groups, (int64_t)activation, eps));
@@ -493,15 +558,21 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
         if (!grads[0].defined()) return variable_list(6);
         const variable_list saved = ctx->get_saved_variables();
+        const double scale = ctx->saved_data["scale"].toDouble();
+        const bool want_q = ctx->needs_input_grad(0), want_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
         variable_list gradients;
-        {
-            const at::AutoDispatchBelowADInplaceOrView below;
-            AttentionCall call(saved[0], saved[1], saved[2], saved[3], saved[4], ctx->saved_data["scale"].toDouble());
-            gradients = call.backward(grads[0], saved[5], saved[6], saved[7], ctx->needs_input_grad(0), ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
+        if (beyond_here(grads[0]))
+            gradients = applied("_CrossAttentionBackward", grads[0], saved[0], saved[1], saved[2], saved[5], saved[6], saved[7], saved[3], saved[4], scale, want_q, want_kv);
+        else {
+            {
+                const at::AutoDispatchBelowADInplaceOrView below;
+                AttentionCall call(saved[0], saved[1], saved[2], saved[3], saved[4], scale);
+                gradients = call.backward(grads[0], saved[5], saved[6], saved[7], want_q, want_kv);
+            }
+            gradients = once(std::move(gradients), "cross_attention is not differentiable twice", saved, grads[0]);
         }
         for (int i = 0; i < 3; ++i)
             if (!ctx->needs_input_grad(i)) gradients[i] = Tensor();
-        gradients = once(std::move(gradients), "cross_attention is not differentiable twice", saved, grads[0]);
         gradients.resize(6);
         return gradients;
     }
@@ -509,10 +580,11 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
 
 std::optional<double> scale_of(PyObject *o) { return o == Py_None ? std::nullopt : std::optional<double>(number(o)); }
 
-// cross_attention(q, k, v, lengths, mask, scale) -> out
+// cross_attention(q, k, v, lengths, mask, scale) -> out, or None: to go through the dispatcher
 PyObject *cross_attention_(PyObject *const *arg) {
     const Tensor &q = tensor(arg[0], "q"), &k = tensor(arg[1], "k"), &v = tensor(arg[2], "v");
     const Tensor lengths = optional(arg[3], "lengths"), mask = optional(arg[4], "mask");
+    if (watched({&q, &k, &v, &lengths, &mask})) return none();
     const std::optional<double> scale = scale_of(arg[5]);
     if (recorded({&q, &k, &v})) return THPVariable_Wrap(AttentionNode::apply(q, k, v, if_there(lengths), if_there(mask), scale));
     AttentionCall call(q, k, v, lengths, mask, scale);
@@ -531,6 +603,9 @@ PyObject *cross_attention_backward_(PyObject *const *arg) {
     return tuple_of({g[0], g[1], g[2]});
 }
 
+// watched(tensor) -> bool
+PyObject *watched_(PyObject *const *arg) { return PyBool_FromLong(watched({&tensor(arg[0], "the argument")})); }
+
 template <Py_ssize_t N, PyObject *(*F)(PyObject *const *)> PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (n != N) {
         PyErr_Format(PyExc_TypeError, "takes %zd arguments, got %zd", N, n);
@@ -548,6 +623,7 @@ template <Py_ssize_t N, PyObject *(*F)(PyObject *const *)> PyObject *entry(PyObj
 PyMethodDef methods[] = {
     {"solve", (PyCFunction)(void (*)())entry<N_ARGS, solve_>, METH_FASTCALL, "One whole solve with a built-in term (see torchode_amd.adjoints)."},
     {"stage", (PyCFunction)(void (*)())entry<7, stage_>, METH_FASTCALL, "One stage around a user's right-hand side (see torchode_amd.adjoints)."},
+    {"watched", (PyCFunction)(void (*)())entry<1, watched_>, METH_FASTCALL, "Whether a tracer or a mode looks on at operations on this tensor."},
     {"group_norm", (PyCFunction)(void (*)())entry<8, group_norm_>, METH_FASTCALL, "See torchode_amd.field_ops."},
     {"group_norm_forward", (PyCFunction)(void (*)())entry<8, group_norm_forward_>, METH_FASTCALL, "The same with its statistics."},
     {"group_norm_backward", (PyCFunction)(void (*)())entry<11, group_norm_backward_>, METH_FASTCALL, "Its vector-Jacobian products."},

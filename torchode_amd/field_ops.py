@@ -5,7 +5,7 @@
 tensors on the GPU, one or two hand-written kernels each (``csrc/tode_norm.hip``, ``csrc/tode_attention.hip``), with gradients:
 an ``f`` that calls them goes wherever an ``f`` of torch operations goes -- ``AutoDiffAdjoint`` with and without gradients, HIP
 graphs of its iterations (``graph_iterations``), both backsolve adjoints (``BacksolveAdjoint`` calls ``f`` one sample at a time under
-``vmap``: shape the state with ``y.reshape(-1, ...)`` there), ``torch.compile`` of ``f``.  Samples stay independent of each other, as
+``vmap``: shape the state with ``y.reshape(-1, ...)`` there), ``torch.compile`` of ``f``, ``torch.jit.trace`` and ``make_fx``.  Samples stay independent of each other, as
 the solver takes them to be.
 
 Neither is differentiable twice or in forward mode: both are refused (``NotImplementedError``, ``RuntimeError`` from PyTorch).  The reference leaves ``f`` to the user (terms.py:13-19).
@@ -20,6 +20,13 @@ from . import _lib
 # A call inside torch.func.vmap, vjp, ... hands out tensors in wrappers: those go through the autograd.Functions below, others through
 # nodes of the extension (csrc/tode_host.cpp).
 _transformed = torch._C._are_functorch_transforms_active
+
+
+def _ops():
+    """The operators that the dispatcher knows, for programs that something records."""
+    from . import ops
+
+    return ops
 
 
 def _without_tangents(name, *tensors):
@@ -52,13 +59,12 @@ def group_norm(
         raise ValueError(f"group_norm: activation must be one of {list(_lib.ACTIVATIONS)}, got {activation!r}")
     act = _lib.ACTIVATIONS[activation]
     if torch.compiler.is_compiling():
-        from . import ops
-
         _without_tangents("group_norm", x, weight, bias, scale, shift)
-        return ops.group_norm(x, n_groups, weight, bias, scale, shift, act, eps)
+        return _ops().group_norm(x, n_groups, weight, bias, scale, shift, act, eps)
     if _transformed():
         return _GroupNorm.apply(x, weight, bias, scale, shift, n_groups, act, eps)[0]
-    return _lib.load_host().group_norm(x, n_groups, weight, bias, scale, shift, act, eps)
+    y = _lib.load_host().group_norm(x, n_groups, weight, bias, scale, shift, act, eps)
+    return _ops().group_norm(x, n_groups, weight, bias, scale, shift, act, eps) if y is None else y
 
 
 def _first(t, dim, size):
@@ -89,6 +95,8 @@ def _fold_norm(size, dims, x, weight, bias, scale, shift, per_sample):
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(x, weight, bias, scale, shift, n_groups, act, eps):
+        if _lib.load_host().watched(x):
+            return _ops().group_norm_forward(x, n_groups, weight, bias, scale, shift, act, eps)
         return _lib.load_host().group_norm_forward(x, n_groups, weight, bias, scale, shift, act, eps)
 
     @staticmethod
@@ -118,6 +126,8 @@ class _GroupNorm(torch.autograd.Function):
 class _GroupNormBackward(torch.autograd.Function):
     @staticmethod
     def forward(dy, x, mean, rstd, weight, bias, scale, shift, n_groups, act, want):
+        if _lib.load_host().watched(x):
+            return _ops().group_norm_backward(dy, x, mean, rstd, n_groups, weight, bias, scale, shift, act, want)
         return _lib.load_host().group_norm_backward(dy, x, mean, rstd, n_groups, weight, bias, scale, shift, act, want)
 
     @staticmethod
@@ -166,13 +176,12 @@ def cross_attention(
     (``q``, ``k``).  Tensors are read in place, whatever the strides of their first three axes; the values of a head have to lie
     side by side, a tensor where they do not is copied."""
     if torch.compiler.is_compiling():
-        from . import ops
-
         _without_tangents("cross_attention", q, k, v)
-        return ops.cross_attention(q, k, v, lengths, mask, scale)
+        return _ops().cross_attention(q, k, v, lengths, mask, scale)
     if _transformed():
         return _CrossAttention.apply(q, k, v, lengths, mask, scale)[0]
-    return _lib.load_host().cross_attention(q, k, v, lengths, mask, scale)
+    out = _lib.load_host().cross_attention(q, k, v, lengths, mask, scale)
+    return _ops().cross_attention(q, k, v, lengths, mask, scale) if out is None else out
 
 
 def _fold(size, dims, *tensors):
@@ -184,6 +193,8 @@ def _fold(size, dims, *tensors):
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(q, k, v, lengths, mask, scale):
+        if _lib.load_host().watched(q):
+            return _ops().cross_attention_forward(q, k, v, lengths, mask, scale)
         return _lib.load_host().cross_attention_forward(q, k, v, lengths, mask, scale)
 
     @staticmethod
@@ -211,6 +222,8 @@ class _CrossAttention(torch.autograd.Function):
 class _CrossAttentionBackward(torch.autograd.Function):
     @staticmethod
     def forward(grad, q, k, v, out, low, lse, lengths, mask, scale, want_q, want_kv):
+        if _lib.load_host().watched(q):
+            return _ops().cross_attention_backward(grad, q, k, v, out, low, lse, lengths, mask, scale, want_q, want_kv)
         return _lib.load_host().cross_attention_backward(grad, q, k, v, out, low, lse, lengths, mask, scale, want_q, want_kv)
 
     @staticmethod

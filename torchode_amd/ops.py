@@ -86,14 +86,38 @@ def mlp_pack_weights(raw: torch.Tensor, matrix_inputs: int, n_features: int = 64
     return torch.ops.torchode_amd.mlp_pack_weights(raw, matrix_inputs, n_features)
 
 
+def group_norm_forward(x, n_groups, weight, bias, scale, shift, activation, eps):
+    """The result of ``torchode_amd.group_norm``, its means and the reciprocals of its deviations, as one operation of a program that is being recorded."""
+    return torch.ops.torchode_amd.group_norm(x, n_groups, weight, bias, scale, shift, activation, eps)
+
+
 def group_norm(x, n_groups, weight, bias, scale, shift, activation, eps):
-    """``torchode_amd.group_norm`` for programs that PyTorch captures, as ``torch.ops.torchode_amd.group_norm``."""
-    return torch.ops.torchode_amd.group_norm(x, n_groups, weight, bias, scale, shift, activation, eps)[0]
+    return group_norm_forward(x, n_groups, weight, bias, scale, shift, activation, eps)[0]
+
+
+def _where_wanted(gradients, wanted):
+    """A list of the wanted gradients, with None for the others."""
+    left = iter(gradients)
+    return tuple(next(left) if w else None for w in wanted)
+
+
+def group_norm_backward(dy, x, mean, rstd, n_groups, weight, bias, scale, shift, activation, want):
+    wanted = [want >> i & 1 and t is not None for i, t in enumerate((x, weight, bias, scale, shift))]
+    want = sum(1 << i for i in range(5) if wanted[i])
+    return _where_wanted(torch.ops.torchode_amd.group_norm_backward(dy, x, mean, rstd, n_groups, weight, bias, scale, shift, activation, want), wanted)
+
+
+def cross_attention_forward(q, k, v, lengths, mask, scale):
+    """``torchode_amd.cross_attention`` likewise, with what rounding took off the result and its rows' log-sums."""
+    return torch.ops.torchode_amd.cross_attention(q, k, v, lengths, mask, scale)
 
 
 def cross_attention(q, k, v, lengths, mask, scale):
-    """``torchode_amd.cross_attention`` likewise."""
-    return torch.ops.torchode_amd.cross_attention(q, k, v, lengths, mask, scale)[0]
+    return cross_attention_forward(q, k, v, lengths, mask, scale)[0]
+
+
+def cross_attention_backward(grad, q, k, v, out, low, lse, lengths, mask, scale, want_q, want_kv):
+    return _where_wanted(torch.ops.torchode_amd.cross_attention_backward(grad, q, k, v, out, low, lse, lengths, mask, scale, want_q, want_kv), (want_q, want_kv, want_kv))
 
 
 # The operators of a right-hand side (field_ops.py) are registered here, over the same native calls that the eager functions make.
@@ -133,13 +157,8 @@ def _group_norm_context(ctx, inputs, output):
 
 def _group_norm_gradients(ctx, dy, _mean, _rstd):
     x, weight, bias, scale, shift, mean, rstd = ctx.saved_tensors
-    asked = [ctx.needs_input_grad[i] for i in (0, 2, 3, 4, 5)]
-    out = iter(
-        torch.ops.torchode_amd.group_norm_backward(
-            dy, x, mean, rstd, ctx.n_groups, weight, bias, scale, shift, ctx.activation, sum(1 << i for i in range(5) if asked[i])
-        )
-    )
-    dx, *rest = (next(out) if a else None for a in asked)
+    want = sum(1 << i for i, j in enumerate((0, 2, 3, 4, 5)) if ctx.needs_input_grad[j])
+    dx, *rest = group_norm_backward(dy, x, mean, rstd, ctx.n_groups, weight, bias, scale, shift, ctx.activation, want)
     return dx, None, *rest, None, None
 
 
@@ -178,10 +197,8 @@ def _cross_attention_context(ctx, inputs, output):
 
 def _cross_attention_gradients(ctx, grad, _low, _lse):
     want_q, want_k, want_v = ctx.needs_input_grad[:3]
-    want_kv = want_k or want_v
     *saved, lengths, mask = ctx.saved_tensors
-    out = iter(torch.ops.torchode_amd.cross_attention_backward(grad, *saved, lengths, mask, ctx.scale, want_q, want_kv))
-    return tuple(next(out) if wanted else None for wanted in (want_q, want_kv, want_kv)) + (None, None, None)
+    return *cross_attention_backward(grad, *saved, lengths, mask, ctx.scale, want_q, want_k or want_v), None, None, None
 
 
 _cross_attention.register_autograd(_cross_attention_gradients, setup_context=_cross_attention_context)
