@@ -481,3 +481,20 @@ def test_recorded_programs(how):
         got, want = program(*values), f(*values)
         for a, b in zip(*((x,) if torch.is_tensor(x) else x for x in (got, want))):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dim", [0, 1, 2, 3])
+def test_mapped_along_any_axis(dim):
+    t, dy = made((5, (6, 7), 12, 3), torch.float32, params=torch.float32, modulated=False, seed=26)
+    f = lambda x, w, b: to.group_norm(x[None], 3, w, b, activation="silu")[0]
+    pulled = lambda x, g: torch.func.vjp(f, x, t["weight"], t["bias"])[1](g)
+    want = torch.func.vmap(pulled)(t["x"], dy)
+    for x_dim, g_dim in ((dim, dim), (0, dim), (dim, 0)):
+        got = torch.func.vmap(pulled, in_dims=(x_dim, g_dim))(t["x"].movedim(0, x_dim), dy.movedim(0, g_dim))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # one sample for all cotangents, whose own axes are the grid's
+    x = t["x"][0]
+    pull = torch.func.vjp(f, x, t["weight"], t["bias"])[1]
+    got = torch.func.vmap(pull, in_dims=dim)(dy.movedim(0, dim))
+    for a, b in zip(got, zip(*(pull(g) for g in dy))):
+        assert torch.equal(a, torch.stack(b))

@@ -392,12 +392,12 @@ struct NormCall {
         return {y, mean, rstd};
     }
     // of x, weight, bias, scale, shift: undefined where bit i of `want` is not set
-    variable_list backward(const Tensor &dy_, const Tensor &mean, const Tensor &rstd, int64_t want) {
+    variable_list backward(const Tensor &dy_, const Tensor &mean_, const Tensor &rstd_, int64_t want) {
         TORCH_CHECK_VALUE(dy_.sizes() == x.sizes() && dy_.scalar_type() == x.scalar_type() && dy_.device() == x.device(), "group_norm: the cotangent must be like x");
         without_tangent("group_norm's gradient", {&dy_});
-        for (const Tensor *t : {&mean, &rstd})
-            TORCH_CHECK_VALUE(t->dim() == 2 && t->size(0) == a.batch && t->size(1) == a.n_groups && t->is_contiguous() && t->scalar_type() == statistics && t->device() == x.device(), "group_norm: mean and rstd must be [batch, groups] as the forward pass returned them");
-        const Tensor dy = dy_.contiguous();
+        for (const Tensor *t : {&mean_, &rstd_})
+            TORCH_CHECK_VALUE(t->dim() == 2 && t->size(0) == a.batch && t->size(1) == a.n_groups && t->scalar_type() == statistics && t->device() == x.device(), "group_norm: mean and rstd must be [batch, groups] as the forward pass returned them");
+        const Tensor dy = dy_.contiguous(), mean = mean_.contiguous(), rstd = rstd_.contiguous();  // (repeated for mapped cotangents of one sample)
         const c10::DeviceGuard guard(x.device());
         a.dy = dy.data_ptr(), a.mean = mean.data_ptr(), a.rstd = rstd.data_ptr();
         const Tensor *like[5] = {&x, &weight, &bias, &scale, &shift};
@@ -529,10 +529,11 @@ struct AttentionCall {
         return {out, low, lse};
     }
     // of q, k, v: undefined where not wanted
-    variable_list backward(const Tensor &grad_, const Tensor &out, const Tensor &low, const Tensor &lse, bool want_q, bool want_kv) {
-        for (const Tensor *t : {&grad_, &out})
+    variable_list backward(const Tensor &grad_, const Tensor &out_, const Tensor &low_, const Tensor &lse_, bool want_q, bool want_kv) {
+        for (const Tensor *t : {&grad_, &out_})
             TORCH_CHECK_VALUE(t->sizes() == q.sizes() && t->scalar_type() == q.scalar_type() && t->device() == q.device(), "cross_attention: the output and its cotangent must be like q");
-        TORCH_CHECK_VALUE(low.is_contiguous() && low.scalar_type() == q.scalar_type() && low.device() == q.device() && (a.dtype == TODE_F32 ? low.numel() == 0 : low.sizes() == q.sizes()) && out.is_contiguous() && lse.is_contiguous() && lse.sizes() == q.sizes().slice(0, 3) && lse.scalar_type() == at::kFloat && lse.device() == q.device(), "cross_attention: out, low and lse must be as the forward pass returned them");
+        TORCH_CHECK_VALUE(low_.scalar_type() == q.scalar_type() && low_.device() == q.device() && (a.dtype == TODE_F32 ? low_.numel() == 0 : low_.sizes() == q.sizes()) && lse_.sizes() == q.sizes().slice(0, 3) && lse_.scalar_type() == at::kFloat && lse_.device() == q.device(), "cross_attention: out, low and lse must be as the forward pass returned them");
+        const Tensor out = out_.contiguous(), low = low_.contiguous(), lse = lse_.contiguous();  // (repeated for mapped cotangents of one sample)
         without_tangent("cross_attention's gradient", {&grad_});
         const Tensor grad = rows(grad_, a.grad_strides);
         const c10::DeviceGuard guard(q.device());

@@ -144,7 +144,7 @@ class _GroupNormBackward(torch.autograd.Function):
         dy_dim, x_dim, mean_dim, rstd_dim, *dims = in_dims[:8]
         # (every mapped sample has its own gradient of a weight, also of one that they share)
         samples, x, *params = _fold_norm(size, (x_dim, *dims), x, weight, bias, scale, shift, True)
-        dy, mean, rstd = (_first(t, d, size).reshape(size * samples, *t.shape[1 if d is None else 2 :]) for t, d in ((dy, dy_dim), (mean, mean_dim), (rstd, rstd_dim)))
+        dy, mean, rstd = _fold(size, (dy_dim, mean_dim, rstd_dim), dy, mean, rstd)
         out = list(_GroupNormBackward.apply(dy, x, mean, rstd, *params, n_groups, act, want))
         out = [None if g is None else g.reshape(size, samples, *g.shape[1:]) for g in out]
         for i, (t, d) in enumerate(((weight, dims[0]), (bias, dims[1]))):
