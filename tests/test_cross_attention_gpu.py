@@ -521,3 +521,25 @@ def test_recorded_programs(how):
         got, want = program(*values), f(*values)
         for a, b in zip(*((x,) if torch.is_tensor(x) else x for x in (got, want))):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_batched_cotangents(dtype):
+    """As one after the other: autograd.grad with is_grads_batched, a Jacobian, and vmap around autograd.grad."""
+    t, _, _ = made((2, 3, 5, 4, 2, 4), DTYPES[dtype], seed=38)
+    lengths = torch.tensor([5, 3], device="cuda")
+    leaves = [v.requires_grad_() for v in t.values()]
+    call = lambda q, k, v: to.cross_attention(q, k, v, lengths=lengths)
+    out = call(*leaves)
+    grad = torch.randn((6, *out.shape), generator=torch.Generator().manual_seed(1)).to(DTYPES[dtype]).cuda()
+    want = [torch.stack(g) for g in zip(*(torch.autograd.grad(out, leaves, g, retain_graph=True) for g in grad))]
+    got = torch.autograd.grad(out, leaves, grad, is_grads_batched=True, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    (got,) = torch.autograd.grad(out, leaves[1], grad, is_grads_batched=True, retain_graph=True)
+    assert torch.equal(got, want[1])
+    for dim in range(5):
+        got = torch.func.vmap(lambda g: torch.autograd.grad(out, leaves, g, retain_graph=True), in_dims=dim)(grad.movedim(0, dim))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    rows = torch.autograd.functional.jacobian(call, tuple(v.detach() for v in leaves), vectorize=True)
+    one = torch.autograd.functional.jacobian(call, tuple(v.detach() for v in leaves))
+    assert all(torch.equal(a, b) for a, b in zip(rows, one))

@@ -483,6 +483,30 @@ def test_recorded_programs(how):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("kind", [None, "silu"])
+def test_batched_cotangents(kind):
+    """As one after the other: autograd.grad with is_grads_batched, a Jacobian, and vmap around autograd.grad."""
+    shape = (2, (3,), 8, 2)
+    t, _ = made(shape, torch.float32, params=torch.float32, modulated=True, seed=25)
+    leaves = [v.requires_grad_() for v in t.values()]
+    call = lambda x, w, b, s, h: to.group_norm(x, 2, w, b, scale=s, shift=h, activation=kind)
+    y = call(*leaves)
+    dy = torch.randn((5, *y.shape), generator=torch.Generator().manual_seed(1)).cuda()
+    want = [torch.stack(g) for g in zip(*(torch.autograd.grad(y, leaves, g, retain_graph=True) for g in dy))]
+    got = torch.autograd.grad(y, leaves, dy, is_grads_batched=True, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    (got,) = torch.autograd.grad(y, leaves[3], dy, is_grads_batched=True, retain_graph=True)
+    assert torch.equal(got, want[3])
+    for dim in range(3):  # (whichever axis is the mapped one)
+        got = torch.func.vmap(lambda g: torch.autograd.grad(y, leaves, g, retain_graph=True), in_dims=dim)(dy.movedim(0, dim))
+        for name, a, b in zip(t, got, want):
+            # (gradients of shared weights are added up over the samples of one cotangent in another order: two of them, so that it is the same)
+            assert torch.equal(a, b), name
+    rows = torch.autograd.functional.jacobian(call, tuple(v.detach() for v in leaves), vectorize=True)
+    one = torch.autograd.functional.jacobian(call, tuple(v.detach() for v in leaves))
+    assert all(torch.equal(a, b) for a, b in zip(rows, one))
+
+
 @pytest.mark.parametrize("dim", [0, 1, 2, 3])
 def test_mapped_along_any_axis(dim):
     t, dy = made((5, (6, 7), 12, 3), torch.float32, params=torch.float32, modulated=False, seed=26)

@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/LegacyBatchedTensorImpl.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
@@ -288,6 +289,32 @@ variable_list once(variable_list gradients, const char *message, const variable_
     return gradients;
 }
 
+// gradients(cotangent), of a cotangent that torch.autograd.grad(is_grads_batched=True) or a vectorised Jacobian has wrapped for each of those in it: one
+// after the other, as there are few and each is a whole backward pass.
+template <typename F> variable_list each(const Tensor &cotangent, F gradients) {
+    const at::BatchedTensorImpl *const batched = at::maybeGetBatchedImpl(cotangent);
+    if (!batched) return gradients(cotangent);
+    std::vector<int64_t> from, to, sizes;
+    at::BatchDims dims;
+    for (const at::BatchDim &dim : batched->bdims()) {  // (in front, in order of their levels)
+        dims.emplace_back(dim.level(), (int64_t)to.size());
+        from.push_back(dim.dim()), to.push_back((int64_t)to.size()), sizes.push_back(batched->value().size(dim.dim()));
+    }
+    const Tensor all = batched->value().movedim(from, to).flatten(0, (int64_t)to.size() - 1);
+    std::vector<std::vector<Tensor>> found;
+    for (int64_t n = 0; n < all.size(0); ++n) {
+        variable_list one = gradients(all[n]);
+        found.resize(one.size());
+        for (size_t i = 0; i < one.size(); ++i)
+            if (one[i].defined()) found[i].push_back(one[i]);
+    }
+    TORCH_CHECK_VALUE(!found.empty(), "no cotangents");
+    variable_list result(found.size());
+    for (size_t i = 0; i < found.size(); ++i)
+        if (!found[i].empty()) result[i] = at::makeBatched(at::stack(found[i]).unflatten(0, sizes), dims);
+    return result;
+}
+
 // A backward pass that something looks on at, or whose cotangent a transform of torch.func has wrapped: the functions of field_ops.py know both.
 bool beyond_here(const Tensor &cotangent) {
     const auto keys = cotangent.unsafeGetTensorImpl()->key_set();
@@ -436,7 +463,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
             {
                 const at::AutoDispatchBelowADInplaceOrView below;
                 NormCall call(saved[0], saved[1], saved[2], saved[3], saved[4], groups, activation);
-                gradients = call.backward(grads[0], saved[5], saved[6], want);
+                gradients = each(grads[0], [&](const Tensor &dy) { return call.backward(dy, saved[5], saved[6], want); });
             }
             gradients = once(std::move(gradients), "group_norm is not differentiable twice", saved, grads[0]);
         }
@@ -568,7 +595,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
             {
                 const at::AutoDispatchBelowADInplaceOrView below;
                 AttentionCall call(saved[0], saved[1], saved[2], saved[3], saved[4], scale);
-                gradients = call.backward(grads[0], saved[5], saved[6], saved[7], want_q, want_kv);
+                gradients = each(grads[0], [&](const Tensor &grad) { return call.backward(grad, saved[5], saved[6], saved[7], want_q, want_kv); });
             }
             gradients = once(std::move(gradients), "cross_attention is not differentiable twice", saved, grads[0]);
         }
