@@ -543,3 +543,20 @@ def test_batched_cotangents(dtype):
     rows = torch.autograd.functional.jacobian(call, tuple(v.detach() for v in leaves), vectorize=True)
     one = torch.autograd.functional.jacobian(call, tuple(v.detach() for v in leaves))
     assert all(torch.equal(a, b) for a, b in zip(rows, one))
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "grad"])
+@pytest.mark.parametrize("head_dim", [1, 8])
+def test_views_that_are_flagged_negative(which, head_dim):
+    """The imaginary part of a conjugate: its memory holds the values of the other sign."""
+    t, _, grad = made((2, 3, 5, 2, 1, head_dim), torch.float32, seed=39)
+    t["grad"] = grad
+    flagged = {**t, which: torch.complex(torch.zeros_like(t[which]), -t[which]).conj().imag}
+    assert flagged[which].is_neg() and torch.equal(flagged[which], t[which])
+
+    def run(q, k, v, grad):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        out = to.cross_attention(*leaves)
+        return [out.detach(), *torch.autograd.grad(out, leaves, grad)]
+
+    assert all(torch.equal(a, b) for a, b in zip(run(**flagged), run(**t)))

@@ -522,3 +522,19 @@ def test_mapped_along_any_axis(dim):
     got = torch.func.vmap(pull, in_dims=dim)(dy.movedim(0, dim))
     for a, b in zip(got, zip(*(pull(g) for g in dy))):
         assert torch.equal(a, torch.stack(b))
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "scale", "shift", "dy"])
+def test_views_that_are_flagged_negative(which):
+    """The imaginary part of a conjugate: its memory holds the values of the other sign."""
+    t, dy = made((3, (5,), 1, 1), torch.float32, params=torch.float32, modulated=True, seed=27)
+    t["dy"] = dy
+    flagged = {**t, which: torch.complex(torch.zeros_like(t[which]), -t[which]).conj().imag}
+    assert flagged[which].is_neg() and torch.equal(flagged[which], t[which])
+
+    def run(x, weight, bias, scale, shift, dy):
+        leaves = [v.detach().requires_grad_() for v in (x, weight, bias, scale, shift)]
+        y = to.group_norm(leaves[0], 1, leaves[1], leaves[2], scale=leaves[3], shift=leaves[4], activation="silu")
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    assert all(torch.equal(a, b) for a, b in zip(run(**flagged), run(**t)))

@@ -256,6 +256,8 @@ PyObject *tuple_of(std::initializer_list<Tensor> tensors) {
     }
     return result;
 }
+// With its values in memory as they are: the imaginary part of a conjugate is a view with a flag that says negative.
+Tensor as_stored(const Tensor &t) { return t.resolve_neg(); }
 // (a graph node's edges belong to the tensors there are)
 std::optional<Tensor> if_there(const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 bool recorded(std::initializer_list<const Tensor *> tensors) {
@@ -380,7 +382,7 @@ struct NormCall {
         TORCH_CHECK_VALUE(!seen || type == dtype, "group_norm: ", may_be_shared ? "weight and bias" : "scale and shift", " must have the same type");
         TORCH_CHECK_VALUE(t.device() == x.device(), "group_norm: ", name, " is on ", t.device(), ", x on ", x.device());
         dtype = type, seen = true;
-        return t.contiguous();
+        return as_stored(t).contiguous();
     }
     NormCall(const Tensor &x_, const Tensor &weight_, const Tensor &bias_, const Tensor &scale_, const Tensor &shift_, int64_t G, int64_t activation) : x(x_) {
         TORCH_CHECK_VALUE(x.dim() >= 2, "group_norm: x must be [batch, ..., channels], got ", x.sizes());
@@ -394,7 +396,7 @@ struct NormCall {
         scale = parameter(scale_, "scale", false, a.modulation_dtype, modulation), shift = parameter(shift_, "shift", false, a.modulation_dtype, modulation);
         without_tangent("group_norm", {&x, &weight_, &bias_, &scale_, &shift_});
         TORCH_CHECK(x.is_cuda(), NEEDS_GPU, x.device(), "'. There is no CPU implementation to fall back to.");
-        x = x.contiguous();
+        x = as_stored(x).contiguous();
         a.n_groups = (int32_t)G, a.channels = (int32_t)C, a.batch = B, a.positions = 1;
         for (int64_t i = 1; i + 1 < x.dim(); ++i) a.positions *= x.size(i);
         a.x = x.data_ptr();
@@ -424,7 +426,7 @@ struct NormCall {
         without_tangent("group_norm's gradient", {&dy_});
         for (const Tensor *t : {&mean_, &rstd_})
             TORCH_CHECK_VALUE(t->dim() == 2 && t->size(0) == a.batch && t->size(1) == a.n_groups && t->scalar_type() == statistics && t->device() == x.device(), "group_norm: mean and rstd must be [batch, groups] as the forward pass returned them");
-        const Tensor dy = dy_.contiguous(), mean = mean_.contiguous(), rstd = rstd_.contiguous();  // (repeated for mapped cotangents of one sample)
+        const Tensor dy = as_stored(dy_).contiguous(), mean = mean_.contiguous(), rstd = rstd_.contiguous();  // (repeated for mapped cotangents of one sample)
         const c10::DeviceGuard guard(x.device());
         a.dy = dy.data_ptr(), a.mean = mean.data_ptr(), a.rstd = rstd.data_ptr();
         const Tensor *like[5] = {&x, &weight, &bias, &scale, &shift};
@@ -504,7 +506,7 @@ struct AttentionCall {
 
     // any strides will do as long as a row's values lie side by side
     static Tensor rows(const Tensor &t, int64_t (&strides)[3]) {
-        const Tensor r = t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous();
+        const Tensor s = as_stored(t), r = s.stride(3) == 1 || s.size(3) == 1 ? s : s.contiguous();
         for (int i = 0; i < 3; ++i) strides[i] = r.stride(i);
         return r;
     }
