@@ -626,9 +626,12 @@ static ForwardPlan plan_forward(const tode_cross_attention_args &a) {
     ForwardPlan p;
     const long long rows = a.queries * (a.heads / a.kv_heads);
     p.groups = a.batch * a.kv_heads;
-    // float32: also where there are few tiles of 128 rows, each of which would go over the keys one tile after the other (64 samples of 128
-    // rows over 200 keys: 14 us against 19)
-    p.few = a.dtype == TODE_F32 && (rows <= 32 || (a.keys > 64 && p.groups * ((rows + 127) / 128) < 512));
+    // float32: also where there are few tiles of 128 rows, each of which would go over the keys one tile after the other, as long as the
+    // workgroups of 32 rows are all on the chip at once, which takes the more of it the longer the heads are (us in this form and the other one, 128 rows over
+    // 200 keys: heads of 32 values, 192 groups 16.3 and 17.5, 256 groups 19.8 and 17.6; of 64, 128 groups 21.8 and 28.0, 160 groups 36.6 and 28.5; of
+    // 128, 64 groups 28.4 and 48.6, 96 groups 59.9 and 51.2)
+    const long long tiles = p.groups * ((rows + 127) / 128);
+    p.few = a.dtype == TODE_F32 && (rows <= 32 || (a.keys > 64 && tiles <= (a.head_dim <= 32 ? 192 : a.head_dim <= 64 ? 128 : 64)));
     p.token = rows <= 8;  // (10 rows of 80 values, float32: 738 us in two blocks of 8, in the general form 566)
     if (p.token) {
         const int N = a.dtype == TODE_F32 ? 4 : 8;

@@ -427,9 +427,11 @@ static BackwardPlan plan_backward(const tode_cross_attention_args &a) {
     BackwardPlan p;
     const long long rows = a.queries * (a.heads / a.kv_heads);
     p.groups = a.batch * a.kv_heads;
-    // four wavefronts on 32 rows where there are no more, and in float32 where there are few tiles of 128 (64 samples of 128 rows over 200 keys:
-    // 18 us against 22; the second kernel is slower that way)
-    p.few_rows = rows <= 32 || (a.dtype == TODE_F32 && a.keys > 64 && p.groups * ((rows + 127) / 128) < 512);
+    // four wavefronts on 32 rows where there are no more, and in float32 where there are few tiles of 128: as forward, here (us of the whole backward
+    // pass, 128 rows over 200 keys) with heads of 32 values 192 groups 52 either way, 256 groups 63 and 54; of 64, 64 groups 54 and 69, 96 groups 78 and 71; of
+    // 128, 64 groups 98 and 133, 96 groups 149 and 138.  (The second kernel is slower that way.)
+    const long long tiles = p.groups * ((rows + 127) / 128);
+    p.few_rows = rows <= 32 || (a.dtype == TODE_F32 && a.keys > 64 && tiles <= (a.head_dim <= 32 ? 192 : 64));
     p.few_keys = a.keys <= 32;
     p.row_tiles = (int)((rows + (p.few_rows ? 31 : 127)) / (p.few_rows ? 32 : 128));
     p.key_tiles = (int)((a.keys + (p.few_keys ? 31 : 127)) / (p.few_keys ? 32 : 128));
