@@ -17,7 +17,9 @@ namespace tode {
 
 constexpr int NORM_RESIDENT_THREADS = 512;                   // (256 registers each)
 constexpr int NORM_ROW_VECTORS = 256;                        // of a workgroup's part of a row at most: as many groups as values, two sums of each in LDS
-constexpr int NORM_MOST = 32, NORM_MOST_BACKWARD = 8;  // vectors a thread keeps of a tensor: 128 registers, twice 32 (with 16 only one workgroup fits: 65 us against 55)
+// vectors a thread keeps of a tensor: 128 registers, backward twice 32.  (Backward with 16 only one workgroup fits, and with 4 fewer samples: 64 samples of
+// 32 x 32 x 320, bfloat16, 54 us with 8, 69 with 16, 54 with 4; 2048 of 32 x 32 x 64, float32, 355, 528 and 507.)
+constexpr int NORM_MOST = 32, NORM_MOST_BACKWARD = 8;
 
 struct NormShape {
     long long B, S, rows;  // rows: of `period` positions each
@@ -1068,17 +1070,21 @@ static ResidentPlan resident_of(const tode_group_norm_args &a, int most) {
             if (best && m * base * bytes_of(a.dtype) > 64 && n.B * (units / m) < 1024) break;
             best = m;
         }
-        if (!best || best * base * bytes_of(a.dtype) < 32) return p;  // (128 x 128 positions, 16 bytes of each: 33 us, in the general form 22)
+        // (64 float32 samples of 32 channels in 8 groups: 16 384 positions, 16 bytes of each 92 us, in the general form 69; 8192 positions, 32 bytes
+        // of each 32 us, in the general form 39)
+        if (!best || best * base * bytes_of(a.dtype) < 32) return p;
         n.chunk = best * base, n.V = n.chunk / N, n.chunks = units / best;
     }
     p.blocks = (n.B >= 8 ? (n.B + 7) / 8 * 8 : n.B) * n.chunks;
     if (p.blocks > (1ll << 31) - 1) return p;
     if (n.period > 1) most /= 2;  // (which value is the last takes registers too)
     if (n.rows * n.period * n.C * bytes_of(a.dtype) > (1ll << 31)) return p;  // (a thread's place in the sample is a 32-bit number)
-    // up to eight vectors a thread as long as there are two wavefronts a SIMD, else as many threads as there may be
-    // too few workgroups for the chip, of 64 KiB or more each (one float32 sample of 64 x 64 x 128: 18.5 us against 15; 37 float16 samples of
-    // 45 x 53 x 120: 37 against 30)
+    // Too few workgroups for the chip, of more than 64 KiB each (us here and in the general form; float32, 64 channels in 8 groups: parts of 256 KiB, 64
+    // workgroups 18.7 and 17.9, 128 workgroups 22.6 and 24.5; of 94 to 128 KiB, up to 64 workgroups 10 to 11 and 12 to 15, but rows of several positions, 5000 of 6
+    // channels, 16.2 and 13.5, and float64 12.6 and 11.8; float16, 45 x 53 positions of 120 channels in 12, 186 KiB, 96 workgroups 26.5 and 25.0, 192
+    // workgroups 28.7 and 32.9)
     if (p.blocks < 128 && n.rows * n.V > 4096) return p;
+    // up to eight vectors a thread as long as there are two wavefronts a SIMD, else as many threads as there may be
     auto with = [&](int R) {
         const long long lanes = (n.rows + R - 1) / R, threads = (lanes * n.V + 63) / 64 * 64;
         if (threads > NORM_RESIDENT_THREADS) return false;
