@@ -968,7 +968,8 @@ int tode_group_norm_backward(const tode_group_norm_args *args, void *stream);
  *   out[b,i,h,:] = sum_j softmax_j(c q[b,i,h,:] . k[b,j,h',:]) v[b,j,h',:],   h' = h / (heads / kv_heads)
  * and its vector-Jacobian products.  Keys j >= lengths[b] (lengths beyond [0, keys] count as the nearer end) and those whose mask byte
  * is 0 are not read into any result, whatever they hold; a row without any key gets zeros, and passes none on.  Scores, sums and the softmax are
- * float32; weights and score gradients are rounded to the data's type ahead of their matrix products. */
+ * float32; weights (beyond eight rows a head of keys) and score gradients are rounded to the data's type ahead of their matrix products,
+ * float16 ones taken times powers of two that keep them within its range. */
 #define TODE_ATTENTION_MAX_HEAD_DIM 256     /* bfloat16, float16 */
 #define TODE_ATTENTION_MAX_HEAD_DIM_F32 128 /* float32 */
 typedef struct tode_cross_attention_args {

@@ -1,5 +1,8 @@
 // Cross attention, forward: for the 32 queries that a wavefront keeps, one pass over the keys with the running maximum and sum of the
 // softmax.  A score is c q.k; p = 2^(s - m) with s in units of log 2; out = (sum p v) / (sum p), in float32.
+// The matrix instructions take both operands in one type, so for the 16-bit ones p is rounded to it ahead of the product with v (their sum is not): an
+// output is off by 0.0023 of its size in bfloat16 (4 samples of 4096 queries over 4096 keys), where its own rounding alone is 0.0017.  Weights in two parts
+// would spare that for half as many products again.  Up to eight rows a head of keys take the vector units, where p stays float32.
 #include "tode_attention.h"
 
 #ifdef TODE_ATT_TYPE
