@@ -208,7 +208,7 @@ __device__ __forceinline__ void dkv_tiles(const tode_cross_attention_args &a, co
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, h = lane / 32, key = (tile * 4 + wave) * 32 + lane % 32;
     T *const buffer = (T *)lds;                              // [2][q, g][64][STRIDE]
     float *const s_rows = (float *)(buffer + 8 * L::VALUES);  // [2][lse, sum][64]
-    const bool allowed = key < p.keys && p.allowed(key);
+    const bool matter = !KEYS || p.scores_matter(lane), allowed = key < p.keys && p.allowed(key);
     Operand<T, DP> k, v;
     k.load(allowed ? p.key(key) : nullptr, p.D, h);
     if (KEYS) v.load(allowed ? p.value(key) : nullptr, p.D, h);
@@ -217,7 +217,7 @@ __device__ __forceinline__ void dkv_tiles(const tode_cross_attention_args &a, co
 #pragma unroll
     for (int t = 0; t < L::NT; ++t) sum[t] = zero16();
     ColumnUnit<T, L::NT> unit;
-    const int row_tiles = tile * 128 < p.length && (!KEYS || p.scores_matter(lane)) ? (p.rows + ROWS - 1) / ROWS : 0, per_split = (row_tiles + splits - 1) / splits;
+    const int row_tiles = tile * 128 < p.length && matter ? (p.rows + ROWS - 1) / ROWS : 0, per_split = (row_tiles + splits - 1) / splits;
     const int first = split * per_split, last = min(first + per_split, row_tiles);
     Raw<T> q_next[LOADS], g_next[LOADS];
     float row_next = 0;
