@@ -2,13 +2,14 @@
 
 ``group_norm`` normalises a field on grids (channels last), modulates it by the time and applies the activation;
 ``cross_attention`` lets the state of every sample look at what an encoder has said about it.  Both are functions of
-tensors on the GPU, one or two hand-written kernels each (``csrc/tode_norm.hip``, ``csrc/tode_attention.hip``), with gradients:
+tensors on the GPU, a few hand-written kernels each (``csrc/tode_norm.hip``, ``csrc/tode_attention.hip``), with gradients:
 an ``f`` that calls them goes wherever an ``f`` of torch operations goes -- ``AutoDiffAdjoint`` with and without gradients, HIP
 graphs of its iterations (``graph_iterations``), both backsolve adjoints (``BacksolveAdjoint`` calls ``f`` one sample at a time under
-``vmap``: shape the state with ``y.reshape(-1, ...)`` there), ``torch.compile`` of ``f``, ``torch.jit.trace`` and ``make_fx``.  Samples stay independent of each other, as
-the solver takes them to be.
+``vmap``: shape the state with ``y.reshape(-1, ...)`` there), ``torch.compile`` of ``f``, ``torch.jit.trace`` and ``make_fx``.  Samples stay
+independent of each other, as the solver takes them to be.
 
-Neither is differentiable twice or in forward mode: both are refused (``NotImplementedError``, ``RuntimeError`` from PyTorch).  The reference leaves ``f`` to the user (terms.py:13-19).
+Neither is differentiable twice or in forward mode: both are refused, as are ``torch.func.grad`` and ``vjp`` inside of a program that is being
+compiled (by PyTorch, which has no such transforms of operators).  The reference leaves ``f`` to the user (terms.py:13-19).
 """
 from typing import Optional
 
