@@ -83,6 +83,21 @@ template <typename T, int DP> struct Operand {
 #pragma unroll
         for (int i = 0; i < Tile<T, DP>::NC; ++i) c[i] = row_part(row, (2 * i + h) * Raw<T>::N, D);
     }
+    // The same of a row that is there, in memory, for all lanes: zeros where it does not count.  (The lanes stay together on the way: a branch of some
+    // lanes would have the compiler spill what it loads within it, where the registers are as short as for 256 values.)
+    __device__ __forceinline__ void load_if(const T *row, int D, int h, bool counts) {
+        if (D == DP) {
+#pragma unroll
+            for (int i = 0; i < Tile<T, DP>::NC; ++i) c[i].load(row + (2 * i + h) * Raw<T>::N);
+        } else {
+#pragma unroll
+            for (int i = 0; i < Tile<T, DP>::NC; ++i) c[i] = row_part(row, (2 * i + h) * Raw<T>::N, D);
+        }
+#pragma unroll
+        for (int i = 0; i < Tile<T, DP>::NC; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) c[i].w[k] = counts ? c[i].w[k] : 0;
+    }
     // ... of the other sign where the scale is negative, so that larger scores have larger weights
     __device__ __forceinline__ void load_signed(const T *row, int D, int h, bool minus) {
         load(row, D, h);

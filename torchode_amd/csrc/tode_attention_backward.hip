@@ -131,8 +131,9 @@ __global__ void __launch_bounds__(64 * WC * WS) attention_dkv_kernel(tode_cross_
     const int key = (tile * WC + wc) * 32 + lane % 32;
     const bool allowed = key < p.keys && p.allowed(key), matter = p.scores_matter(lane);
     Operand<T, DP> k, v;
-    k.load(allowed ? p.key(key) : nullptr, p.D, h);
-    v.load(allowed ? p.value(key) : nullptr, p.D, h);
+    const int there = min(key, p.keys - 1);
+    k.load_if(p.key(there), p.D, h, allowed);
+    v.load_if(p.value(there), p.D, h, allowed);
     const float c = (float)a.scale * LOG2E;
     acc16 dk[L::NT], dv[L::NT];
 #pragma unroll
