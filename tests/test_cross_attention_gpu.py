@@ -560,3 +560,19 @@ def test_views_that_are_flagged_negative(which, head_dim):
         return [out.detach(), *torch.autograd.grad(out, leaves, grad)]
 
     assert all(torch.equal(a, b) for a, b in zip(run(**flagged), run(**t)))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", [(418, 112, 4, 8, 8, 16), (60, 400, 300, 4, 4, 64), (700, 8, 50, 4, 4, 64), (2, 1, 20000, 16, 4, 64), (16, 500, 900, 4, 2, 128)], ids=ids)
+def test_an_output_and_what_rounding_takes_off_it(shape, dtype):
+    """Their sum is what was there ahead of the rounding, also where that lay in the middle between two steps of the type."""
+    from torchode_amd import _lib
+
+    dtype = DTYPES[dtype]
+    t, _, _ = made(shape, dtype, seed=40)
+    out, low, _ = _lib.load_host().cross_attention_forward(t["q"], t["k"], t["v"], None, None, None)
+    want, size, narrow = field_oracle.cross_attention(dtype, *(t[k].double() for k in "qkv"), None, None, None)["out"]
+    error = (out.double() + low.double() - want).abs()
+    # (the remainder's own rounding: half a step of half a step, and of float16's smallest numbers)
+    tolerance = field_oracle.ROUNDINGS * 2.0**-24 * size + narrow + (torch.finfo(dtype).eps / 2) ** 2 * want.abs() + (2.0**-25 if dtype == torch.float16 else 0)
+    assert (error <= tolerance).all(), ((error / tolerance).max(), int((error > tolerance).sum()))

@@ -8,6 +8,8 @@
 //   forward, gradient of q:  columns are queries, rows keys;  gradients of k and v: columns are keys, rows queries.
 // The G = H / Hkv heads that share a head of keys are rows (columns) of one problem: row r is query r / G of head r % G of the group.
 #pragma once
+#include <type_traits>
+
 #include "tode_field.h"
 
 namespace tode {
@@ -244,6 +246,14 @@ template <typename T, int NT> __device__ __forceinline__ void store_column(T *ro
                 for (int e = 0; e < 4; ++e)
                     if (d + e < D) row[d + e] = v[e];
         }
+}
+
+// A product that is rounded to T twice -- to be written, and for what that takes off -- and has to be the same number both times: the compiler
+// may take a multiplication and the rounding to float16 behind it as one operation with a single rounding, the first time and not the second, and
+// near the middle between two steps the two then differ by a whole one.
+template <typename T> __device__ __forceinline__ float settled(float v) {
+    if (std::is_same<T, f16>::value) asm("" : "+v"(v));
+    return v;
 }
 
 // What rounding to T takes off.

@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(256, CT * DP <= 128 ? 2 : 1) attention_tiles_k
 #pragma unroll
         for (int t = 0; t < L::NT; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) out[ct][t][r] *= f;
+            for (int r = 0; r < 16; ++r) out[ct][t][r] = settled<T>(out[ct][t][r] * f);
         write_columns<T, DP>(p, a.out, own, out[ct], row0 + 32 * ct, lane);
         if (a.out_low) keep_low<T, L::NT>(out[ct]), write_columns<T, DP>(p, a.out_low, own, out[ct], row0 + 32 * ct, lane);
     }
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_short_kernel(tode_cro
 #pragma unroll
         for (int t = 0; t < L::NT; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) out[t][r] *= f;
+            for (int r = 0; r < 16; ++r) out[t][r] = settled<T>(out[t][r] * f);
         if (a.lse && h == 0 && row < p.rows) a.lse[p.flat(row)] = log_sum(m, l);
         write_columns<T, DP>(p, a.out, own, out, row0, lane);
         if (a.out_low) keep_low<T, L::NT>(out), write_columns<T, DP>(p, a.out_low, own, out, row0, lane);
@@ -557,7 +557,7 @@ __global__ void __launch_bounds__(256) attention_token_kernel(tode_cross_attenti
         const float f = reciprocal(l[r]);
         if (a.lse && part == 0) a.lse[p.flat(r)] = log_sum(m[r], l[r]);
 #pragma unroll
-        for (int e = 0; e < N; ++e) out[r][e] *= f;
+        for (int e = 0; e < N; ++e) out[r][e] = settled<T>(out[r][e] * f);
         auto write = [&](void *of) {
             T *const to = (T *)of + p.flat(r) * p.D + part;
             if (whole) {
@@ -613,7 +613,7 @@ template <typename T> __global__ void __launch_bounds__(256) attention_join_kern
     for (int i = 1; i < parts; ++i) v += s_sum[thread + i * wide];
     const int query = row / G;
     const long long at = (b * a.queries + query) * a.heads + (group - b * a.kv_heads) * G + row - query * G;
-    v *= reciprocal(l);
+    v = settled<T>(v * reciprocal(l));
     ((T *)a.out)[at * D + d] = (T)v;
     if (a.out_low) ((T *)a.out_low)[at * D + d] = (T)(v - (float)(T)v);
     if (a.lse && thread == 0) a.lse[at] = log_sum(top, l);
