@@ -538,3 +538,12 @@ def test_views_that_are_flagged_negative(which):
         return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
 
     assert all(torch.equal(a, b) for a, b in zip(run(**flagged), run(**t)))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_float32_gradients_of_the_parameters_of_16_bit_data(dtype, kind):
+    """One position a sample: a gradient of the shift is a single product, and float32."""
+    shape = (2000, (1,), 64, 2)
+    t, dy = made(shape, DTYPES[dtype], params=torch.float32, modulated=True, seed=28)
+    check(shape, DTYPES[dtype], kind, t, dy)

@@ -66,17 +66,17 @@ template <bool SHORT> __device__ __forceinline__ double tangent(double z) { retu
 
 // The normal distribution's function and density times sqrt(2 pi).  The tail is density times a polynomial in t = 1 / (1 + c |z|): its ratio to
 // the density falls slowly and is smooth in t.  Coefficients by weighted least squares to the smallest relative error for |z| < 14, where the
-// density ends: 6e-6 for 16 bits, 2e-8 for float32, whose |z| < 1 take an odd polynomial about 1/2 instead (4e-8 of it; differences from 1 would
-// double the error).  One power and one reciprocal; erfcf takes several times as long (512 float32 samples of 64 x 64 x 16: 76 us; 66 with five
-// coefficients for everything, which were off by 7e-8 of 1 and by a tenth of a per cent at -4; 37 float16 ones of 45 x 53 x 120: 30).
+// density ends: 1.5e-7 for 16 bits (whose parameters may have float32 gradients), 2e-8 for float32, whose |z| < 1 take an odd polynomial about 1/2
+// instead (4e-8 of it; differences from 1 would double the error).  One power and one reciprocal; erfcf takes several times as long (512 float32 samples of 64 x 64 x 16: 76 us; 66 with five
+// coefficients for everything, which were off by 7e-8 of 1 and by a tenth of a per cent at -4; 37 float16 ones of 45 x 53 x 120: 31).
 template <bool SHORT> __device__ __forceinline__ void normal(float z, float &below, float &density) {
     const float x = fabsf(z), s = z * z;
     density = __builtin_amdgcn_exp2f(s * -0.72134752044448170368f);
-    const float t = __builtin_amdgcn_rcpf(fmaf(x, SHORT ? 0.3125f : 0.2625f, 1.0f));
+    const float t = __builtin_amdgcn_rcpf(fmaf(x, SHORT ? 0.3f : 0.2625f, 1.0f));
     float p;
     if (SHORT) {
-        p = fmaf(-0.0720064332f, t, 0.169261103f), p = fmaf(p, t, 0.0257095609f), p = fmaf(p, t, 0.129970966f);
-        p = fmaf(p, t, 0.122265234f), p = fmaf(p, t, 0.124796638f);
+        p = fmaf(0.0355736409f, t, -0.156781816f), p = fmaf(p, t, 0.205628049f), p = fmaf(p, t, -0.0530165609f), p = fmaf(p, t, 0.128209209f);
+        p = fmaf(p, t, 0.100020071f), p = fmaf(p, t, 0.120736926f), p = fmaf(p, t, 0.119630405f);
     } else {
         p = fmaf(0.0306574329f, t, -0.148385007f), p = fmaf(p, t, 0.233887704f), p = fmaf(p, t, -0.132396963f), p = fmaf(p, t, 0.148453724f);
         p = fmaf(p, t, 0.0561404901f), p = fmaf(p, t, 0.102743951f), p = fmaf(p, t, 0.104149397f), p = fmaf(p, t, 0.104749262f);
