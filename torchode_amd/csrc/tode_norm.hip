@@ -141,8 +141,8 @@ template <int N, bool SHORT, typename A> __device__ __forceinline__ void activat
 }
 
 // f(act) with act known to the compiler.  A loop that is unrolled for values in registers has the code of one activation in a row that way, and not
-// that of all of them between any two of its steps, which is more than the instruction cache holds (512 float32 samples of 64 x 64 x 16 with SiLU: 60 us, 76 the other way; 128 bfloat16 ones of
-// 64 x 64 x 256: 142 against 150).
+// that of all of them between any two of its steps, which is more than the instruction cache holds (512 float32 samples of 64 x 64 x 16 with
+// SiLU: 60 us, 76 the other way; 128 bfloat16 ones of 64 x 64 x 256: 142 against 150).
 template <typename F> __device__ __forceinline__ void with_activation(int act, F f) {
     switch (act) {
         case TODE_ACT_SILU: f(std::integral_constant<int, TODE_ACT_SILU>()); break;

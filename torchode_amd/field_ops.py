@@ -174,7 +174,8 @@ def cross_attention(
 
     Types: float32 (``D`` up to 128), bfloat16, float16 (up to 256).  Scores, softmax and sums are float32; with the latter two
     the softmax's weights (and in the backward pass the scores' gradients) are rounded to the data's type ahead of the product with ``v``
-    (``q``, ``k``), float16 ones in a range of their own; not the weights of up to eight rows (queries times the heads that share a head of keys).  Tensors are read in place, whatever the strides of their first three axes; the values of a head have to lie
+    (``q``, ``k``), float16 ones in a range of their own; the weights of up to eight rows (queries times the heads that share a head of
+    keys) are not.  Tensors are read in place, whatever the strides of their first three axes; the values of a head have to lie
     side by side, a tensor where they do not is copied."""
     if torch.compiler.is_compiling():
         _without_tangents("cross_attention", q, k, v)
